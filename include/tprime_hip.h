@@ -33,6 +33,7 @@ extern "C" {
 #define TP_BF16 0
 #define TP_F16 1
 #define TP_F32 2
+#define TP_FP8 3 /* float8_e4m3fn; key-value caches only */
 
 /* Library version (major*10000 + minor*100 + patch). */
 int tp_version(void);
@@ -425,6 +426,62 @@ int tp_embedding_fwd(const void* table, const int64_t* ids, void* out, int64_t n
 int tp_embedding_bwd(const void* dout, const int64_t* ids, void* dtable, int64_t n, int vocab, int hidden, int dtype, void* stream);
 
 int tp_linears(const tp_linear_problem* problems, int count, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Answering with a model: a paged key-value cache, attention of one new token over it, sampling.
+ * (The reference trains only; these have no counterpart there.)
+ *
+ * tp_kv_cache: position t of sequence b lies in page table[b * table_stride + t / page_size], slot t % page_size; a page
+ * holds page_size (a power of two from 8 up) rows of k_dim keys and v_dim values for each of `heads` kv heads, at
+ * (page, head, slot) element strides.  dtype TP_BF16 / TP_F16 / TP_F32 stores rows as they are; TP_FP8 stores
+ * e4m3(x * (448 / a)) with a = max |x| of the row and keeps a / 448 in k_scale / v_scale (pages, heads, page_size), contiguous
+ * (rows with a < 2^-100 become zeros; rows with an infinity or a NaN read back as NaN).  A table entry outside [0, pages)
+ * names no page: nothing is stored there, zeros are read, and attention leaves its positions out.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct tp_kv_cache {
+  void *k, *v;
+  float *k_scale, *v_scale; /* NULL unless dtype is TP_FP8 */
+  const int32_t* table;     /* (sequences, table_width) */
+  int64_t table_stride;
+  int64_t k_strides[3], v_strides[3];
+  int table_width, pages, page_size, heads, k_dim, v_dim, dtype;
+} tp_kv_cache;
+
+/* Stores the rows of S tokens of each of B sequences: k (B, heads, S, k_dim) and v (B, heads, S, v_dim) at (batch, head, token)
+ * strides; token s of sequence b goes to position positions[b] + s, for s < counts[b] (counts NULL: all S).  Positions
+ * outside the table are left out.  dtype: that of k and v, the cache's own, or a 16-bit one for a TP_FP8 cache. */
+int tp_kv_cache_write(const tp_kv_cache* cache, const void* k, const void* v, const int32_t* positions,
+                      const int32_t* counts, int B, int S, const int64_t k_strides[3], const int64_t v_strides[3],
+                      int dtype, void* stream);
+
+/* The first L positions of each sequence laid out in rows: k (B, heads, L, k_dim), v (B, heads, L, v_dim) of type dtype,
+ * zeros from position lengths[b] on. */
+int tp_kv_cache_read(const tp_kv_cache* cache, const int32_t* lengths, void* k, void* v, int B, int L,
+                     const int64_t k_strides[3], const int64_t v_strides[3], int dtype, void* stream);
+
+/* Attention of the newest token of each sequence, whose row is already in the cache, over the cached positions
+ * j in [max(0, lengths[b] - 1 - window_left), lengths[b])  (window_left < 0: all):
+ *   out[b, h] = sum_j softmax_j(cap(sm_scale * q[b, h] . k_j)) v_j,   cap(x) = soft_cap * tanh(x / soft_cap)  (0: none)
+ * q (B, Hq, k_dim), out (B, Hq, v_dim) at (batch, head) strides, lse (B, Hq) fp32 contiguous (natural log; may be NULL);
+ * a sequence of length 0 gets zeros and an lse of -inf.  ws: tp_paged_attn_workspace_bytes bytes, 16-byte aligned. */
+size_t tp_paged_attn_workspace_bytes(const tp_kv_cache* cache, int B, int Hq, int dtype);
+int tp_paged_attn(const tp_kv_cache* cache, const void* q, const int32_t* lengths, void* out, float* lse, void* ws, int B,
+                  int Hq, const int64_t q_strides[2], const int64_t o_strides[2], float sm_scale, int window_left,
+                  float soft_cap, int dtype, void* stream);
+
+/* The next token of each of B rows of V <= 2^18 logits, row_stride elements apart, drawn with the given uniform[b] in [0, 1):
+ *   l = logit (NaN: -inf), m = max l, w = 2^((l - m) * (log2(e) / temperature)), 1 where l == m, rounded to a multiple of 2^-35
+ *   K: the first top_k tokens by falling l, the lower index first among equals (top_k <= 0: all)
+ *   P: the shortest beginning of K with at least top_p of its weight, never empty;  kept: those of P with w >= min_p
+ *   token: the first kept one, by index, with a sum of kept weights up to itself above uniform * (sum of all kept);
+ *   logprob: log(w / sum of all kept)
+ * A temperature that is not positive takes the first of the largest logits.  A row without a logit above -inf gives token -1 and
+ * logprob -inf.  Each of temperatures, top_ks, top_ps, min_ps is (B) or NULL: then the value beside it holds for all rows.
+ * ws: tp_sample_workspace_bytes bytes (may be 0), 16-byte aligned. */
+size_t tp_sample_workspace_bytes(int B, int V);
+int tp_sample(const void* logits, const float* uniform, const float* temperatures, const int32_t* top_ks,
+              const float* top_ps, const float* min_ps, float temperature, int top_k, float top_p, float min_p,
+              int64_t* tokens, float* logprobs, void* ws, int B, int V, int64_t row_stride, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

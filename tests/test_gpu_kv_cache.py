@@ -1,0 +1,240 @@
+"""The paged key-value cache: rows stored in pages and read back, bit for bit (stored as they are, or in 8 bits with a scale),
+and nothing else touched."""
+
+import pytest
+import torch
+
+from tests.util import randn
+from torchprime_amd import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+FP8 = torch.float8_e4m3fn
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def bits(t):
+  return t.contiguous().view({1: torch.uint8, 2: torch.int16, 4: torch.int32}[t.element_size()]).cpu()
+
+
+def new_cache(pages, H, page, D, dtype, slots_first=False, seed=0, fill=None):
+  shape = (pages, page, H, D) if slots_first else (pages, H, page, D)
+  x = randn(shape, seed) if fill is None else torch.full(shape, fill)
+  x = x.to(dtype)
+  return x.transpose(1, 2) if slots_first else x
+
+
+def table_for(B, width, pages, seed):
+  g = torch.Generator().manual_seed(seed)
+  return torch.randperm(pages, generator=g)[: B * width].reshape(B, width).to(torch.int32)
+
+
+def quantised(x):
+  """What the 8-bit cache holds for rows x, every step rounded once in fp32: (stored, scale)."""
+  x = x.float()
+  top = x.abs().amax(-1)
+  some = top >= 2.0**-100
+  scale = torch.where(some, top / 448.0, torch.zeros(()))
+  back = torch.where(some, torch.full_like(top, 448.0) / top, torch.zeros(()))  # (torch takes 448.0 / top as a reciprocal and a product)
+  finite = torch.isfinite(x).all(-1)
+  y = torch.where(finite[..., None], x * back[..., None], torch.zeros(()))
+  return y.to(FP8), torch.where(finite, scale, torch.full((), float("nan")))
+
+
+def stored(cache, scale, rows, table, positions, counts):
+  """The cache after rows (B,H,S,D) went in: one place after the other."""
+  cache, scale = cache.clone(), None if scale is None else scale.clone()
+  page = cache.shape[2]
+  values, s = (rows.to(cache.dtype), None) if scale is None else quantised(rows)
+  raw, vraw = (cache, values) if scale is None else (cache.view(torch.uint8), values.view(torch.uint8))
+  for b in range(rows.shape[0]):
+    for i in range(rows.shape[2] if counts is None else min(int(counts[b]), rows.shape[2])):
+      t = int(positions[b]) + i
+      if t < 0 or t // page >= table.shape[1] or not 0 <= table[b, t // page] < cache.shape[0]:
+        continue
+      raw[table[b, t // page], :, t % page] = vraw[b, :, i]
+      if scale is not None:
+        scale[table[b, t // page], :, t % page] = s[b, :, i]
+  return cache, scale
+
+
+def check_write(B, S, H, Dk, Dv, page, dtype, quant=False, slots_first=False, counts=None, positions=None, width=None, edit=None, seed=1,
+                rows_of=None):
+  positions = positions if positions is not None else [(7 * b + 3) % (2 * page) for b in range(B)]
+  width = width or -(-(max(positions) + S) // page)
+  pages = B * width + 2
+  table = table_for(B, width, pages, seed)
+  if edit:
+    edit(table)
+  make = rows_of or (lambda d, sd: randn((B, S, H, d), sd).transpose(1, 2))
+  k, v = make(Dk, seed + 1).to(dtype), make(Dv, seed + 2).to(dtype)
+  cdt = FP8 if quant else dtype
+  kc, vc = new_cache(pages, H, page, Dk, cdt, slots_first, seed + 3), new_cache(pages, H, page, Dv, cdt, slots_first, seed + 4)
+  ks, vs = (randn((pages, H, page), seed + 5).abs(), randn((pages, H, page), seed + 6).abs()) if quant else (None, None)
+  pos = torch.tensor(positions, dtype=torch.int32)
+  cnt = None if counts is None else torch.tensor(counts, dtype=torch.int32)
+  dev = lambda t: None if t is None else t.to(DEV)  # noqa: E731  (keeps strides)
+  got = [dev(t) for t in (kc, vc, ks, vs)]
+  assert ops.kv_cache_write(dev(k), dev(v), got[0], got[1], dev(table), dev(pos), dev(cnt), k_scale=got[2], v_scale=got[3]) is None
+  want_k, want_ks = stored(kc, ks, k, table, positions, counts)
+  want_v, want_vs = stored(vc, vs, v, table, positions, counts)
+  for name, g, w in (("k", got[0], want_k), ("v", got[1], want_v), ("k_scale", got[2], want_ks), ("v_scale", got[3], want_vs)):
+    if w is None:
+      continue
+    g, w = g.cpu(), w
+    same = (bits(g) == bits(w)) | (torch.isnan(g.float()) & torch.isnan(w.float())).view(bits(g).shape)
+    assert bool(same.all()), f"{name}: {(~same).sum()} of {same.numel()} differ"
+
+
+@pytest.mark.parametrize("quant,dtype", [(False, BF16), (False, F16), (False, F32), (True, BF16), (True, F16)])
+@pytest.mark.parametrize("B,S,H,Dk,Dv,page,slots_first", [
+  (1, 1, 1, 64, 64, 8, False), (3, 1, 8, 128, 128, 64, False), (2, 37, 3, 128, 128, 16, True), (2, 130, 2, 192, 128, 32, False),
+  (5, 3, 2, 72, 8, 8, True), (1, 9, 1, 512, 256, 8, False),
+])  # fmt: skip
+def test_rows_go_to_their_places(B, S, H, Dk, Dv, page, slots_first, quant, dtype):
+  check_write(B, S, H, Dk, Dv, page, dtype, quant, slots_first)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_counts_and_places_outside_are_left_out(quant):
+  def holes(table):
+    table[0, 1] = -1
+    table[2, 0] = 1000  # beyond the cache
+
+  check_write(4, 20, 2, 64, 64, 8, BF16, quant, counts=[20, 0, 13, 50], positions=[0, 5, 3, 30], width=5, edit=holes)
+  check_write(2, 6, 2, 64, 64, 8, BF16, quant, positions=[-3, 2**31 - 3], width=2)
+
+
+def test_rows_with_extremes_in_8_bits():
+  """Rows of zeros, of tiny and huge values, of exact halves, and with an infinity or a NaN in them; the others stay clean."""
+  def rows(d, seed):
+    x = randn((1, 12, 2, d), seed)
+    x[0, 0] = 0.0
+    x[0, 1] *= 1e-36
+    x[0, 2] *= 2.0**-101
+    x[0, 3] *= 1e30
+    x[0, 4, :, 5] = float("inf")
+    x[0, 5, :, 6] = float("nan")
+    x[0, 6, 0, 0] = -float("inf")
+    x[0, 7] = (torch.arange(2 * d).reshape(2, d) % 449) / 448.0
+    x[0, 8] = torch.arange(2 * d).reshape(2, d).float() - d
+    x[0, 9, :, :] = -0.0
+    x[0, 10, :, 3] = 3e38
+    return x.transpose(1, 2)
+
+  check_write(1, 12, 2, 128, 64, 8, BF16, True, rows_of=rows)
+  check_write(1, 12, 2, 128, 64, 8, BF16, False, rows_of=rows)
+
+
+def test_every_16_bit_value_is_rounded_as_in_32_bits():
+  """All bfloat16 values from -448 to 448 beside a 448, so that the scale is 1 and the stored value e4m3(x) itself."""
+  x = torch.arange(-2**15, 2**15, dtype=torch.int32).to(torch.int16).view(BF16)
+  x = x[torch.isfinite(x) & (x.abs() <= 448)]
+  x = torch.cat([x, x[: -len(x) % 127]]).view(-1, 127)
+  x = torch.cat([x, torch.full((len(x), 1), 448.0, dtype=BF16)], 1)
+  S = x.shape[0]
+  check_write(1, S, 1, 128, 128, 64, BF16, True, positions=[0], rows_of=lambda d, seed: x[None, None])
+
+
+def test_views_odd_addresses_and_long_tables():
+  """k and v as slices of a larger tensor and one element off a 16-byte address; int64 positions and table; a table that is a view."""
+  B, S, H, D, page = 2, 5, 2, 64, 8
+  both = randn((B, S, 2 * H + 1, D), 3, BF16).to(DEV)
+  k, v = both[:, :, :H].transpose(1, 2), both[:, :, H : 2 * H].transpose(1, 2)
+  off = torch.empty(B * H * S * D + 1, dtype=BF16, device=DEV)[1:].view(B, H, S, D).copy_(v)
+  table = table_for(B, 4, 10, 5).to(DEV)
+  for tab, vv, pos in ((table[:, 1:3], v, torch.tensor([3, 0], device=DEV)), (table[:, :2].long(), off, torch.tensor([3, 0], dtype=torch.int32, device=DEV)),
+                       (table.t().contiguous().t(), off, torch.tensor([3, 0], device=DEV))):  # fmt: skip
+    kc, vc = torch.zeros((10, H, page, D), dtype=BF16, device=DEV), torch.zeros((10, H, page, D), dtype=BF16, device=DEV)
+    ops.kv_cache_write(k, vv, kc, vc, tab, pos)
+    want, _ = stored(torch.zeros((10, H, page, D), dtype=BF16), None, v.cpu(), tab.cpu(), [3, 0], None)
+    assert torch.equal(vc.cpu(), want)
+    ko, vo = ops.kv_cache_read(kc, vc, tab, pos + S, 8)
+    assert torch.equal(vo[0, :, 3:8], v[0]) and torch.equal(ko[1, :, :5], k[1]) and (vo[1, :, 5:] == 0).all()
+
+
+@pytest.mark.parametrize("cache,out", [(BF16, BF16), (F16, F16), (F32, F32), (FP8, BF16), (FP8, F16)])
+@pytest.mark.parametrize("B,H,Dk,Dv,page,width,L,lengths,slots_first", [
+  (1, 1, 64, 64, 8, 1, 1, [1], False), (3, 2, 128, 128, 16, 4, 61, [61, 0, 17], False), (2, 3, 192, 128, 64, 2, 100, [100, 64], True),
+  (2, 1, 8, 72, 8, 3, 40, [30, 24], False),
+])  # fmt: skip
+def test_read_back(B, H, Dk, Dv, page, width, L, lengths, slots_first, cache, out):
+  pages = B * width + 1
+  table = table_for(B, width, pages, 2)
+  kc, vc = (new_cache(pages, H, page, d, cache, slots_first, 3 + d) for d in (Dk, Dv))
+  scales = [randn((pages, H, page), 9 + i).abs() if cache == FP8 else None for i in range(2)]
+  got = ops.kv_cache_read(kc.to(DEV), vc.to(DEV), table.to(DEV), torch.tensor(lengths, device=DEV), L, dtype=out,
+                          k_scale=None if scales[0] is None else scales[0].to(DEV), v_scale=None if scales[1] is None else scales[1].to(DEV))
+  for g, c, s, d in zip(got, (kc, vc), scales, (Dk, Dv)):
+    assert g.shape == (B, H, L, d) and g.dtype == out
+    want = torch.zeros((B, H, L, d), dtype=out)
+    for b in range(B):
+      for t in range(min(lengths[b], L, width * page)):
+        x = c[table[b, t // page], :, t % page]
+        want[b, :, t] = x if s is None else (x.float() * s[table[b, t // page], :, t % page, None]).to(out)
+    assert torch.equal(bits(g), bits(want))
+
+
+def test_read_of_what_no_page_holds_is_zero():
+  kc = torch.full((2, 1, 8, 64), float("nan"), dtype=BF16, device=DEV)
+  table = torch.tensor([[-1, 7], [2, -1]], dtype=torch.int32, device=DEV)
+  k, v = ops.kv_cache_read(kc, kc, table, torch.tensor([16, 40], device=DEV), 40)
+  assert (k == 0).all() and (v == 0).all()
+  k, v = ops.kv_cache_read(kc, kc, table, torch.tensor([-1, 0], device=DEV), 0)
+  assert k.shape == (2, 1, 0, 64)
+
+
+def test_offsets_beyond_32_bits():
+  """Pages whose elements lie past 2^32 in the cache (8-bit, 4.3 GB) and past 2^31 bytes (bfloat16)."""
+  H, page, D = 8, 128, 128
+  per = H * page * D
+  pages = (2**32 + 2**24) // per
+  kc = torch.zeros((pages, H, page, D), dtype=torch.uint8, device=DEV).view(FP8)
+  ks = torch.zeros((pages, H, page), device=DEV)
+  table = torch.tensor([[pages - 1, 3]], dtype=torch.int32, device=DEV)
+  x = randn((1, H, 140, D), 4, BF16)
+  ops.kv_cache_write(x.to(DEV), x.to(DEV), kc, kc.clone(), table, torch.zeros(1, dtype=torch.int32, device=DEV), k_scale=ks, v_scale=ks.clone())
+  want, scale = quantised(x)
+  last = torch.full((), pages - 1)
+  assert torch.equal(kc[last].view(torch.uint8).cpu(), want[0, :, :128].view(torch.uint8)) and torch.equal(ks[last].cpu(), scale[0, :, :128])
+  assert torch.equal(kc[3, :, :12].view(torch.uint8).cpu(), want[0, :, 128:].view(torch.uint8))
+  assert int((ks != 0).sum()) == H * 140
+  k, _ = ops.kv_cache_read(kc, kc, table, torch.tensor([140], device=DEV), 140, k_scale=ks, v_scale=ks)
+  assert torch.equal(k.cpu(), (want.float() * scale[..., None]).to(BF16))
+
+
+def test_refusals():
+  H, page, D = 2, 8, 64
+  kc = torch.zeros((4, H, page, D), dtype=BF16, device=DEV)
+  f8, sc = torch.zeros((4, H, page, D), dtype=torch.uint8, device=DEV).view(FP8), torch.zeros((4, H, page), device=DEV)
+  k = torch.zeros((1, H, 3, D), dtype=BF16, device=DEV)
+  table, pos = torch.zeros((1, 2), dtype=torch.int32, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+  W = ops.kv_cache_write
+  for err, call in (
+    (ValueError, lambda: W(k, k, kc[:, :1], kc[:, :1], table, pos)),
+    (ValueError, lambda: W(k, k[..., :32], kc, kc, table, pos)),
+    (ValueError, lambda: W(k[0], k[0], kc, kc, table, pos)),
+    (ValueError, lambda: W(k, k, kc, kc, table[0], pos)),
+    (ValueError, lambda: W(k, k, kc, kc, table, pos.expand(2))),
+    (ValueError, lambda: W(k, k, kc.transpose(2, 3), kc.transpose(2, 3), table, pos)),
+    (ValueError, lambda: W(k, k, f8, f8, table, pos)),
+    (ValueError, lambda: W(k, k, kc, kc, table, pos, k_scale=sc, v_scale=sc)),
+    (ValueError, lambda: W(k, k, f8, f8, table, pos, k_scale=sc[:2], v_scale=sc)),
+    (ValueError, lambda: W(k, k, kc.view(-1)[: 3 * H * page * D + 8][8:].view(3, H, page, D)[..., 1:33], kc[:3, ..., :32], table, pos)),
+    (TypeError, lambda: W(k, k, kc, kc.float(), table, pos)),
+    (TypeError, lambda: W(k, k, kc, kc, table.float(), pos)),
+    (TypeError, lambda: W(k, k, kc, kc, table, pos.float())),
+    (TypeError, lambda: W(k, k, f8, f8, table, pos, k_scale=sc.half(), v_scale=sc.half())),
+    (NotImplementedError, lambda: W(k.half(), k.half(), kc, kc, table, pos)),
+    (NotImplementedError, lambda: W(k.float(), k.float(), f8, f8, table, pos, k_scale=sc, v_scale=sc)),
+    (NotImplementedError, lambda: W(k, k, kc.view(4, H, 4, 2 * D)[..., :D], kc.view(4, H, 4, 2 * D)[..., :D], table, pos)),
+    (NotImplementedError, lambda: W(k.clone().requires_grad_(), k, kc, kc, table, pos)),
+    (NotImplementedError, lambda: ops.kv_cache_read(kc, kc, table, pos, 4, dtype=F16)),
+    (NotImplementedError, lambda: ops.kv_cache_read(f8, f8, table, pos, 4, dtype=F32, k_scale=sc, v_scale=sc)),
+    (ValueError, lambda: ops.kv_cache_read(kc, kc, table, pos, -1)),
+    (ValueError, lambda: ops.kv_cache_read(kc, kc, table, pos[0], 4)),
+    (RuntimeError, lambda: W(k, k, kc, kc, table.cpu(), pos)),
+  ):  # fmt: skip
+    with pytest.raises(err):
+      call()
+  assert (kc == 0).all()

@@ -15,7 +15,7 @@ import torch  # noqa: F401  (loads the HIP runtime the library links against)
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtprime_hip.so")
 
-TP_BF16, TP_F16, TP_F32 = 0, 1, 2
+TP_BF16, TP_F16, TP_F32, TP_FP8 = 0, 1, 2, 3
 _DTYPE_CODE = {torch.bfloat16: TP_BF16, torch.float16: TP_F16, torch.float32: TP_F32}
 
 _I64x3 = c_int64 * 3
@@ -34,6 +34,12 @@ class AttnBwdProblem(ctypes.Structure):  # tp_attn_bwd_problem
 class AttnBwdPlan(ctypes.Structure):  # tp_attn_bwd_plan
   _fields_ = [("parts_bytes", c_size_t), ("sizes", ctypes.c_int32 * 8)]
   _fields_ += [(n, ctypes.c_int32) for n in ("queue", "cap", "sums_at")] + [("first", ctypes.c_uint16 * 65), ("tile", ctypes.c_uint8 * 64)]
+
+
+class KvCache(ctypes.Structure):  # tp_kv_cache
+  _fields_ = [(n, c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table")] + [("table_stride", c_int64)]
+  _fields_ += [("k_strides", _I64x3), ("v_strides", _I64x3)]
+  _fields_ += [(n, c_int) for n in ("table_width", "pages", "page_size", "heads", "k_dim", "v_dim", "dtype")]
 
 
 # name -> (restype, argtypes); every symbol the header declares
@@ -106,6 +112,12 @@ SIGNATURES = {
   "tp_attn_pairs_fit": (c_int, [c_int] * 5),
   "tp_mask_pairs": (c_int, [c_void_p, c_int64 * 2] + [c_int] * 4 + [c_void_p, c_int, c_void_p]),
   "tp_attn_fwd_pairs": (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 2 + [c_int] * 7 + [_I64x3] * 4 + [c_float, c_int, c_void_p]),
+  "tp_kv_cache_write": (c_int, [c_void_p] * 5 + [c_int] * 2 + [_I64x3] * 2 + [c_int, c_void_p]),
+  "tp_kv_cache_read": (c_int, [c_void_p] * 4 + [c_int] * 2 + [_I64x3] * 2 + [c_int, c_void_p]),
+  "tp_paged_attn_workspace_bytes": (c_size_t, [c_void_p] + [c_int] * 3),
+  "tp_paged_attn": (c_int, [c_void_p] * 6 + [c_int] * 2 + [c_int64 * 2] * 2 + [c_float, c_int, c_float, c_int, c_void_p]),
+  "tp_sample_workspace_bytes": (c_size_t, [c_int] * 2),
+  "tp_sample": (c_int, [c_void_p] * 6 + [c_float, c_int, c_float, c_float] + [c_void_p] * 3 + [c_int] * 2 + [c_int64, c_int, c_void_p]),
   "tp_attn_bwd_parts_bytes": (c_size_t, [c_void_p]),
   "tp_attn_bwd_make_plan": (c_size_t, [c_void_p, c_void_p]),
   "tp_attn_bwd_run": (c_int, [c_void_p, c_void_p]),

@@ -1,5 +1,8 @@
-// Error plumbing and version query shared by every entry point of libtprime_hip.so.
-#include "common.hpp"
+// What every entry point of libtprime_hip.so shares (error plumbing, version query), and the operators that answer with a model:
+// the paged key-value cache, attention over it, sampling.
+#include "kv_cache.hpp"
+#include "paged_attn.hpp"
+#include "sample.hpp"
 
 namespace tp {
 

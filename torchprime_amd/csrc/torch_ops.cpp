@@ -171,6 +171,10 @@ TP_OP(swiglu_fwd, Tensor(const Tensor&, const Tensor&))
 TP_OP(swiglu_bwd, T2(const Tensor&, const Tensor&, const Tensor&))
 TP_OP(cross_entropy_fwd, T3(const Tensor&, const Tensor&, int64_t, bool))
 TP_OP(cross_entropy_bwd, Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t))
+TP_OP(kv_cache_write, void(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, OptTensor, OptTensor, OptTensor))
+TP_OP(kv_cache_read, T2(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, at::ScalarType, OptTensor, OptTensor))
+TP_OP(paged_attn, T2(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, double, int64_t, double, OptTensor, OptTensor))
+TP_OP(sample, T2(const Tensor&, const Tensor&, OptTensor, OptTensor, OptTensor, OptTensor, double, int64_t, double, double))
 
 // ---- autograd plumbing -----------------------------------------------------------------------------------------
 // A node with its saved tensors in one array.  ``bwd`` runs the backward operator: below autograd in an ordinary
@@ -1487,6 +1491,164 @@ std::optional<Tensor> py_llama_head(const Tensor& x, const Tensor& residual, con
   return logits;
 }
 
+// ---- the paged key-value cache, attention over it, sampling ------------------------------------------------------------
+// A cache is (pages, heads, page_size, dim) tensors at any strides, a table of pages per sequence, and for 8 bits a scale per
+// row.  Caches are written in place and may be most of the card's memory: what the kernels cannot take as it lies is refused,
+// never copied.
+int cache_code(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? TP_FP8 : dtype_code(t); }
+
+// prep_heads, for tensors that may be contiguous and still start at any address
+Tensor prep_rows(const Tensor& t) {
+  const Tensor h = prep_heads(t);
+  return at16(h) ? h : h.clone(at::MemoryFormat::Contiguous);
+}
+struct Cache {
+  tp_kv_cache c{};
+  Tensor table;  // keeps a copy alive
+};
+Tensor prep_int(const Tensor& t, int64_t B, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == B, name, " must have shape (", B, ",), got (", t.sizes(), ")");
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64, got ", t.scalar_type());
+  return t.to(at::kInt).contiguous();
+}
+Cache prep_cache(const Tensor& k, const Tensor& v, const Tensor& table, int64_t B, const Tensor& k_scale, const Tensor& v_scale) {
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 4 && k.size(0) == v.size(0) && k.size(1) == v.size(1) && k.size(2) == v.size(2), "k_cache (", k.sizes(),
+                    ") and v_cache (", v.sizes(), ") must be (pages, heads, page_size, dim) with the same pages, heads and page_size");
+  TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), "k_cache and v_cache differ in dtype: ", k.scalar_type(), ", ", v.scalar_type());
+  TORCH_CHECK_VALUE(k.numel() && v.numel(), "the cache is empty");
+  TORCH_CHECK_VALUE(k.stride(3) == 1 && v.stride(3) == 1, "the cache's last dimension must be contiguous");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(0) == B && table.size(1) > 0, "block_table must have shape (", B, ", pages per sequence), got (", table.sizes(), ")");
+  TORCH_CHECK_TYPE(table.scalar_type() == at::kInt || table.scalar_type() == at::kLong, "block_table must be int32 or int64, got ", table.scalar_type());
+  const bool quant = k.scalar_type() == at::kFloat8_e4m3fn;
+  for (const Tensor* s : {&k_scale, &v_scale}) {
+    TORCH_CHECK_VALUE(s->defined() == quant, quant ? "an 8-bit cache needs k_scale and v_scale" : "k_scale and v_scale go with an 8-bit cache only");
+    if (!quant) continue;
+    TORCH_CHECK_TYPE(s->scalar_type() == at::kFloat, "the scales must be float32, got ", s->scalar_type());
+    TORCH_CHECK_VALUE(s->is_contiguous() && s->sizes() == k.sizes().slice(0, 3), "the scales must be contiguous (", k.sizes().slice(0, 3), "), got (", s->sizes(), ")");
+  }
+  Cache r;
+  r.table = table.to(at::kInt);
+  if (r.table.stride(1) != 1) r.table = r.table.contiguous();
+  r.c.k = k.data_ptr();
+  r.c.v = v.data_ptr();
+  r.c.k_scale = (float*)opt_ptr(k_scale);
+  r.c.v_scale = (float*)opt_ptr(v_scale);
+  r.c.table = (const int32_t*)r.table.data_ptr();
+  r.c.table_stride = r.table.stride(0);
+  for (int i = 0; i < 3; i++) {
+    r.c.k_strides[i] = k.stride(i);
+    r.c.v_strides[i] = v.stride(i);
+  }
+  const auto narrow = [](int64_t n) { TORCH_CHECK_NOT_IMPLEMENTED(n < (1ll << 31), "a size of ", n, " is too large"); return (int)n; };
+  r.c.table_width = narrow(r.table.size(1));
+  r.c.pages = narrow(k.size(0));
+  r.c.heads = narrow(k.size(1));
+  r.c.page_size = narrow(k.size(2));
+  r.c.k_dim = narrow(k.size(3));
+  r.c.v_dim = narrow(v.size(3));
+  r.c.dtype = cache_code(k.scalar_type());
+  return r;
+}
+
+void kv_cache_write_cuda(const Tensor& k_, const Tensor& v_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& positions_,
+                         OptTensor counts_, OptTensor k_scale, OptTensor v_scale) {
+  const c10::Device dev = require_gpu(k_, v_, k_cache, v_cache, table, positions_, counts_, k_scale, v_scale);
+  c10::DeviceGuard guard(dev);
+  TORCH_CHECK_VALUE(k_.dim() == 4 && v_.dim() == 4, "k and v must be (batch, heads, tokens, dim)");
+  const int64_t B = k_.size(0), H = k_.size(1), S = k_.size(2);
+  const Cache c = prep_cache(k_cache, v_cache, table, B, val(k_scale), val(v_scale));
+  TORCH_CHECK_VALUE(v_.size(0) == B && v_.size(1) == H && v_.size(2) == S && H == c.c.heads && k_.size(3) == c.c.k_dim && v_.size(3) == c.c.v_dim, "k (",
+                    k_.sizes(), ") and v (", v_.sizes(), ") do not fit caches of (", k_cache.sizes(), ") and (", v_cache.sizes(), ")");
+  TORCH_CHECK_TYPE(k_.scalar_type() == v_.scalar_type(), "k and v differ in dtype: ", k_.scalar_type(), ", ", v_.scalar_type());
+  const Tensor positions = prep_int(positions_, B, "positions"), counts = counts_.has_value() ? prep_int(*counts_, B, "counts") : undef();
+  if (B == 0 || S == 0) return;
+  const Tensor k = prep_rows(k_), v = prep_rows(v_);
+  const Strides3 ks = strides3(k), vs = strides3(v);
+  check(tp_kv_cache_write(&c.c, k.data_ptr(), v.data_ptr(), (const int32_t*)positions.data_ptr(), (const int32_t*)opt_ptr(counts), (int)B, (int)S,
+                          ks.data(), vs.data(), dtype_code(k.scalar_type()), stream_of(dev)), "tp_kv_cache_write");
+}
+// what is cached carries no gradient: asking for one is a mistake that would otherwise pass in silence
+void kv_cache_write_autograd(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& positions,
+                             OptTensor counts, OptTensor k_scale, OptTensor v_scale) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::compute_requires_grad(k, v, k_cache, v_cache),
+                              "kv_cache_write has no derivative: call it under torch.no_grad() or detach its inputs");
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    op_kv_cache_write()(k, v, k_cache, v_cache, table, positions, counts, k_scale, v_scale);
+  }
+  for (const Tensor& t : {k_cache, v_cache, val(k_scale), val(v_scale)})
+    if (t.defined() && !t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
+T2 kv_cache_read_cuda(const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths_, int64_t max_length, at::ScalarType dtype,
+                      OptTensor k_scale, OptTensor v_scale) {
+  const c10::Device dev = require_gpu(k_cache, v_cache, table, lengths_, k_scale, v_scale);
+  c10::DeviceGuard guard(dev);
+  TORCH_CHECK_VALUE(lengths_.dim() == 1, "lengths must have shape (batch,), got (", lengths_.sizes(), ")");
+  const int64_t B = lengths_.size(0);
+  const Cache c = prep_cache(k_cache, v_cache, table, B, val(k_scale), val(v_scale));
+  TORCH_CHECK_VALUE(max_length >= 0 && max_length < (1ll << 31), "max_length must lie in [0, 2^31), got ", max_length);
+  const Tensor lengths = prep_int(lengths_, B, "lengths");
+  Tensor k = at::empty({B, c.c.heads, max_length, c.c.k_dim}, k_cache.options().dtype(dtype));
+  Tensor v = at::empty({B, c.c.heads, max_length, c.c.v_dim}, k_cache.options().dtype(dtype));
+  if (k.numel()) {
+    const Strides3 ks = strides3(k), vs = strides3(v);
+    check(tp_kv_cache_read(&c.c, (const int32_t*)lengths.data_ptr(), k.data_ptr(), v.data_ptr(), (int)B, (int)max_length, ks.data(), vs.data(),
+                           dtype_code(dtype), stream_of(dev)), "tp_kv_cache_read");
+  }
+  return {k, v};
+}
+
+T2 paged_attn_cuda(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths_, double sm_scale,
+                   int64_t window_left, double soft_cap, OptTensor k_scale, OptTensor v_scale) {
+  const c10::Device dev = require_gpu(q_, k_cache, v_cache, table, lengths_, k_scale, v_scale);
+  c10::DeviceGuard guard(dev);
+  TORCH_CHECK_VALUE(q_.dim() == 4 && q_.size(2) == 1, "q must be (batch, heads, 1, dim), got (", q_.sizes(), ")");
+  const int64_t B = q_.size(0), Hq = q_.size(1);
+  const Cache c = prep_cache(k_cache, v_cache, table, B, val(k_scale), val(v_scale));
+  TORCH_CHECK_VALUE(q_.size(3) == c.c.k_dim, "q (", q_.sizes(), ") does not fit a k_cache of (", k_cache.sizes(), ")");
+  TORCH_CHECK_VALUE(Hq > 0 && Hq % c.c.heads == 0, "num query heads ", Hq, " must be a multiple of num kv heads ", c.c.heads);
+  const Tensor lengths = prep_int(lengths_, B, "lengths"), q = prep_rows(q_);
+  Tensor out = empty_like_heads(q, c.c.v_dim), lse = empty_f32({B, Hq, 1}, q);
+  if (B) {
+    const int dt = dtype_code(q.scalar_type());
+    const size_t bytes = tp_paged_attn_workspace_bytes(&c.c, (int)B, (int)Hq, dt);
+    const Tensor ws = bytes ? empty_f32({(int64_t)(bytes / 4)}, q) : undef();
+    const int64_t qs[2] = {q.stride(0), q.stride(1)}, os[2] = {out.stride(0), out.stride(1)};
+    check(tp_paged_attn(&c.c, q.data_ptr(), (const int32_t*)lengths.data_ptr(), out.data_ptr(), (float*)lse.data_ptr(), opt_ptr(ws), (int)B, (int)Hq, qs,
+                        os, (float)sm_scale, (int)std::clamp<int64_t>(window_left, -1, 0x7fffffff), (float)soft_cap, dt, stream_of(dev)), "tp_paged_attn");
+  }
+  return {out, lse};
+}
+
+T2 sample_cuda(const Tensor& logits_, const Tensor& uniform_, OptTensor temperatures_, OptTensor top_ks_, OptTensor top_ps_, OptTensor min_ps_,
+               double temperature, int64_t top_k, double top_p, double min_p) {
+  const c10::Device dev = require_gpu(logits_, uniform_, temperatures_, top_ks_, top_ps_, min_ps_);
+  c10::DeviceGuard guard(dev);
+  TORCH_CHECK_VALUE(logits_.dim() == 2 && logits_.size(1) > 0, "logits must be (batch, vocabulary), got (", logits_.sizes(), ")");
+  const int64_t B = logits_.size(0), V = logits_.size(1);
+  const auto per_row = [&](OptTensor t, const char* name) {
+    if (!t.has_value()) return undef();
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == B, name, " must have shape (", B, ",), got (", t->sizes(), ")");
+    TORCH_CHECK_TYPE(t->is_floating_point(), name, " must be of a floating type, got ", t->scalar_type());
+    return t->to(at::kFloat).contiguous();
+  };
+  const Tensor u = per_row(uniform_, "uniform"), ts = per_row(temperatures_, "temperature"), ps = per_row(top_ps_, "top_p"), ms = per_row(min_ps_, "min_p");
+  const Tensor ks = top_ks_.has_value() ? prep_int(*top_ks_, B, "top_k") : undef();
+  const Tensor logits = logits_.stride(1) == 1 && (B == 1 || logits_.stride(0) >= V) ? logits_ : logits_.contiguous();
+  Tensor tokens = at::empty({B}, logits.options().dtype(at::kLong)), logprobs = empty_f32({B}, logits);
+  if (B) {
+    TORCH_CHECK_NOT_IMPLEMENTED(B < (1ll << 31) && V < (1ll << 31), "logits of (", logits.sizes(), ") are too large");
+    const size_t bytes = tp_sample_workspace_bytes((int)B, (int)V);
+    const Tensor ws = bytes ? empty_f32({(int64_t)(bytes / 4)}, logits) : undef();
+    check(tp_sample(logits.data_ptr(), (const float*)u.data_ptr(), (const float*)opt_ptr(ts), (const int32_t*)opt_ptr(ks), (const float*)opt_ptr(ps),
+                    (const float*)opt_ptr(ms), (float)temperature, (int)std::clamp<int64_t>(top_k, 0, 0x7fffffff), (float)top_p, (float)min_p,
+                    (int64_t*)tokens.data_ptr(), (float*)logprobs.data_ptr(), opt_ptr(ws), (int)B, (int)V, B == 1 ? V : logits.stride(0),
+                    dtype_code(logits.scalar_type()), stream_of(dev)), "tp_sample");
+  }
+  return {tokens, logprobs};
+}
+
 // ---- Python entry points -----------------------------------------------------------------------------------------
 // What the Python functions of ops.py call: the GPU check with its own message, then the operator.
 Tensor py_rmsnorm(const Tensor& x, const Tensor& w, double eps) { require_gpu(x, w); return std::get<0>(op_rmsnorm_fwd()(x, w, eps)); }
@@ -1538,6 +1700,26 @@ int64_t py_mask_verdict(const Tensor& mask) {
 Tensor py_l2norm(const Tensor& x, double eps) { return std::get<0>(op_l2norm_fwd()(x, eps)); }
 Tensor py_swiglu(const Tensor& g, const Tensor& u) { return op_swiglu_fwd()(g, u); }
 Tensor py_cross_entropy(const Tensor& l, const Tensor& y, int64_t ignore) { return std::get<0>(op_cross_entropy_fwd()(l, y, ignore, true)); }
+void py_kv_cache_write(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& positions,
+                       OptTensor counts, OptTensor k_scale, OptTensor v_scale) {
+  require_gpu(k, v, k_cache, v_cache, table, positions, counts, k_scale, v_scale);
+  op_kv_cache_write()(k, v, k_cache, v_cache, table, positions, counts, k_scale, v_scale);
+}
+T2 py_kv_cache_read(const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths, int64_t max_length, at::ScalarType dtype,
+                    OptTensor k_scale, OptTensor v_scale) {
+  require_gpu(k_cache, v_cache, table, lengths, k_scale, v_scale);
+  return op_kv_cache_read()(k_cache, v_cache, table, lengths, max_length, dtype, k_scale, v_scale);
+}
+Tensor py_paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table, const Tensor& lengths, double sm_scale,
+                          int64_t window_left, double soft_cap, OptTensor k_scale, OptTensor v_scale) {
+  require_gpu(q, k_cache, v_cache, table, lengths, k_scale, v_scale);
+  return std::get<0>(op_paged_attn()(q, k_cache, v_cache, table, lengths, sm_scale, window_left, soft_cap, k_scale, v_scale));
+}
+T2 py_sample(const Tensor& logits, const Tensor& uniform, OptTensor temperatures, OptTensor top_ks, OptTensor top_ps, OptTensor min_ps, double temperature,
+             int64_t top_k, double top_p, double min_p) {
+  require_gpu(logits, uniform, temperatures, top_ks, top_ps, min_ps);
+  return op_sample()(logits, uniform, temperatures, top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p);
+}
 
 }  // namespace
 
@@ -1565,6 +1747,14 @@ TORCH_LIBRARY(tprime, m) {
   m.def("swiglu_bwd(Tensor dout, Tensor gate, Tensor up) -> (Tensor, Tensor)");
   m.def("cross_entropy_fwd(Tensor logits, Tensor labels, int ignore_index, bool scored_only=False) -> (Tensor, Tensor, Tensor)");
   m.def("cross_entropy_bwd(Tensor dloss, Tensor logits, Tensor labels, Tensor lse, Tensor loss_and_count, int ignore_index) -> Tensor");
+  m.def("kv_cache_write(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor positions, Tensor? counts=None, "
+        "Tensor(c!)? k_scale=None, Tensor(d!)? v_scale=None) -> ()");
+  m.def("kv_cache_read(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lengths, int max_length, ScalarType dtype, Tensor? k_scale=None, "
+        "Tensor? v_scale=None) -> (Tensor, Tensor)");
+  m.def("paged_attn(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lengths, float sm_scale, int window_left=-1, "
+        "float soft_cap=0., Tensor? k_scale=None, Tensor? v_scale=None) -> (Tensor, Tensor)");
+  m.def("sample(Tensor logits, Tensor uniform, Tensor? temperatures, Tensor? top_ks, Tensor? top_ps, Tensor? min_ps, float temperature, int top_k, "
+        "float top_p, float min_p) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(tprime, CUDA, m) {
@@ -1587,6 +1777,10 @@ TORCH_LIBRARY_IMPL(tprime, CUDA, m) {
   m.impl("swiglu_bwd", swiglu_bwd_cuda);
   m.impl("cross_entropy_fwd", cross_entropy_fwd_cuda);
   m.impl("cross_entropy_bwd", cross_entropy_bwd_cuda);
+  m.impl("kv_cache_write", kv_cache_write_cuda);
+  m.impl("kv_cache_read", kv_cache_read_cuda);
+  m.impl("paged_attn", paged_attn_cuda);
+  m.impl("sample", sample_cuda);
 }
 
 TORCH_LIBRARY_IMPL(tprime, Autograd, m) {
@@ -1600,7 +1794,8 @@ TORCH_LIBRARY_IMPL(tprime, Autograd, m) {
   m.impl("scale_rows", scale_rows_autograd);
   m.impl("swiglu_fwd", swiglu_fwd_autograd);
   m.impl("cross_entropy_fwd", cross_entropy_fwd_autograd);
-  for (const char* name : {"rope_table", "rmsnorm_bwd", "add_rmsnorm_bwd", "attn_bwd", "attn_bwd_masked", "attn_bwd_pairs", "l2norm_bwd",
+  m.impl("kv_cache_write", kv_cache_write_autograd);
+  for (const char* name : {"kv_cache_read", "paged_attn", "sample", "rope_table", "rmsnorm_bwd", "add_rmsnorm_bwd", "attn_bwd", "attn_bwd_masked", "attn_bwd_pairs", "l2norm_bwd",
                            "swiglu_bwd", "cross_entropy_bwd"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
 }
@@ -1629,4 +1824,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("l2norm", &py_l2norm, no_gil);
   m.def("swiglu", &py_swiglu, no_gil);
   m.def("cross_entropy", &py_cross_entropy, no_gil);
+  m.def("kv_cache_write", &py_kv_cache_write, no_gil);
+  m.def("kv_cache_read", &py_kv_cache_read, no_gil);
+  m.def("paged_attention", &py_paged_attention, no_gil);
+  m.def("sample", &py_sample, no_gil);
 }

@@ -38,6 +38,10 @@ __all__ = [
   "swiglu",
   "cross_entropy",
   "cross_entropy_fwd",
+  "kv_cache_write",
+  "kv_cache_read",
+  "paged_attention",
+  "sample",
 ]
 
 # the operators themselves (with all their outputs), for callers below autograd and for traces
@@ -52,6 +56,9 @@ l2norm_fwd, l2norm_bwd = _ops.l2norm_fwd.default, _ops.l2norm_bwd.default
 scale_rows = _ops.scale_rows.default
 swiglu_fwd, swiglu_bwd = _ops.swiglu_fwd.default, _ops.swiglu_bwd.default
 cross_entropy_fwd, cross_entropy_bwd = _ops.cross_entropy_fwd.default, _ops.cross_entropy_bwd.default
+
+kv_cache_write_op, kv_cache_read_op = _ops.kv_cache_write.default, _ops.kv_cache_read.default
+paged_attn, sample_op = _ops.paged_attn.default, _ops.sample.default
 
 
 # ------------------------------------------------------------------------------------------------
@@ -174,6 +181,28 @@ def _(dloss, logits, labels, lse, loss_and_count, ignore_index):
   return torch.empty_like(logits, memory_format=torch.contiguous_format)
 
 
+@torch.library.register_fake("tprime::kv_cache_write")
+def _(k, v, k_cache, v_cache, block_table, positions, counts=None, k_scale=None, v_scale=None):
+  return None
+
+
+@torch.library.register_fake("tprime::kv_cache_read")
+def _(k_cache, v_cache, block_table, lengths, max_length, dtype, k_scale=None, v_scale=None):
+  rows = (lengths.shape[0], k_cache.shape[1], max_length)
+  return k_cache.new_empty((*rows, k_cache.shape[3]), dtype=dtype), k_cache.new_empty((*rows, v_cache.shape[3]), dtype=dtype)
+
+
+@torch.library.register_fake("tprime::paged_attn")
+def _(q, k_cache, v_cache, block_table, lengths, sm_scale, window_left=-1, soft_cap=0.0, k_scale=None, v_scale=None):
+  return _empty_like_heads(q, v_cache.shape[-1]), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+
+@torch.library.register_fake("tprime::sample")
+def _(logits, uniform, temperatures, top_ks, top_ps, min_ps, temperature, top_k, top_p, min_p):
+  B = logits.shape[0]
+  return logits.new_empty((B,), dtype=torch.int64), logits.new_empty((B,), dtype=torch.float32)
+
+
 # ------------------------------------------------------------------------------------------------
 # what users call
 # ------------------------------------------------------------------------------------------------
@@ -287,3 +316,89 @@ def cross_entropy(logits: Tensor, labels: Tensor, ignore_index: int) -> Tensor:
   if is_compiling() or overridden(logits, labels):
     return cross_entropy_fwd(logits, labels, ignore_index, True)[0]
   return _native.cross_entropy(logits, labels, ignore_index)
+
+
+# ------------------------------------------------------------------------------------------------
+# answering with a model: a paged key-value cache, attention over it, sampling
+# ------------------------------------------------------------------------------------------------
+# A cache is k_cache (pages, Hkv, page_size, Dqk) and v_cache (pages, Hkv, page_size, Dv) at any strides with a contiguous last
+# dimension and 16-byte rows, page_size a power of two from 8 up.  Position t of sequence b lies in page
+# block_table[b, t // page_size], slot t % page_size; an entry that names no page (-1) holds nothing.  A float8_e4m3fn cache has
+# k_scale and v_scale (pages, Hkv, page_size) in float32: a row is stored as x * (448 / max|x|), its scale is max|x| / 448.
+def kv_cache_write(
+  k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, positions: Tensor, counts: Tensor | None = None,
+  *, k_scale: Tensor | None = None, v_scale: Tensor | None = None,
+) -> None:  # fmt: skip
+  """Stores new keys (B,Hkv,S,Dqk) and values (B,Hkv,S,Dv): token s of sequence b at position ``positions[b] + s``, for
+  s < ``counts[b]`` (None: all S).  Positions outside the table and entries that name no page are left out.
+
+  No two stored tokens may have the same place.  There is no derivative: call it under ``torch.no_grad()``."""
+  args = (k, v, k_cache, v_cache, block_table, positions, counts, k_scale, v_scale)
+  if is_compiling() or overridden(*args):
+    kv_cache_write_op(*args)
+  else:
+    _native.kv_cache_write(*args)
+
+
+def kv_cache_read(
+  k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor, max_length: int, *, dtype: torch.dtype | None = None,
+  k_scale: Tensor | None = None, v_scale: Tensor | None = None,
+) -> tuple[Tensor, Tensor]:  # fmt: skip
+  """The first ``max_length`` positions of each sequence as (B,Hkv,max_length,D) tensors, zeros from ``lengths[b]`` on.
+  ``dtype``: theirs, for a float8 cache (default bfloat16; float16); any other cache is read in its own type."""
+  if dtype is None:
+    dtype = torch.bfloat16 if k_cache.dtype == torch.float8_e4m3fn else k_cache.dtype
+  args = (k_cache, v_cache, block_table, lengths, max_length, dtype, k_scale, v_scale)
+  if is_compiling() or overridden(k_cache, v_cache, block_table, lengths, k_scale, v_scale):
+    return kv_cache_read_op(*args)
+  return _native.kv_cache_read(*args)
+
+
+def paged_attention(
+  q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor, sm_scale: float | None = None,
+  *, window_left: int | None = None, soft_cap: float | None = None, k_scale: Tensor | None = None, v_scale: Tensor | None = None,
+) -> Tensor:  # fmt: skip
+  """Attention of the newest token of each sequence, q (B,Hq,1,Dqk), over its ``lengths[b]`` cached positions (its own among
+  them): (B,Hq,1,Dv).  A sequence of length 0 gets zeros.
+
+  ``sm_scale=None`` means ``1/sqrt(Dv)``, as in ``attention``.  ``window_left``: only positions ``j >= lengths[b] - 1 -
+  window_left``.  ``soft_cap``: logits become ``cap * tanh(logits / cap)``."""
+  if soft_cap is not None and soft_cap <= 0:
+    raise ValueError(f"soft_cap must be positive, got {soft_cap}")
+  if window_left is not None and window_left < 0:
+    raise ValueError(f"window_left must not be negative, got {window_left}")
+  if sm_scale is None:
+    sm_scale = 1.0 / math.sqrt(v_cache.shape[-1])
+  args = (q, k_cache, v_cache, block_table, lengths, sm_scale, -1 if window_left is None else window_left, float(soft_cap or 0.0), k_scale, v_scale)
+  if is_compiling() or overridden(q, k_cache, v_cache, block_table, lengths, k_scale, v_scale):
+    return paged_attn(*args)[0]
+  return _native.paged_attention(*args)
+
+
+def sample(
+  logits: Tensor, uniform: Tensor, temperature: float | Tensor = 1.0, top_k: int | Tensor = 0, top_p: float | Tensor = 1.0,
+  min_p: float | Tensor = 0.0,
+) -> tuple[Tensor, Tensor]:  # fmt: skip
+  """The next token of each row of ``logits`` (B, V), drawn with ``uniform`` (B) in [0, 1), and its log-probability in the
+  distribution that it was drawn from: (B) int64, (B) float32.  The settings are numbers, or tensors (B) of one per row.
+
+  Tokens are ranked by falling logit, the lower index first among equals.  Of the softmax of ``logits / temperature`` the first
+  ``top_k`` are kept (0 or less: all); of those the fewest first that have ``top_p`` of their weight, at least one; of those the
+  ones with at least ``min_p`` times the largest weight.  The draw takes the first kept token, by index, whose cumulative weight
+  exceeds ``uniform`` times the whole.  A temperature that is not positive takes the largest logit.  NaN logits count as -inf; a
+  row of nothing else gives token -1 and log-probability -inf.
+
+  Weights are held on a grid of 2^-35 of the largest, on which their sums are exact: the same inputs give the same token, always."""
+  rows, numbers = [], []
+  for name, x, off, ok in (
+    ("temperature", temperature, 1.0, lambda x: x >= 0), ("top_k", top_k, 0, lambda x: True),
+    ("top_p", top_p, 1.0, lambda x: 0 <= x <= 1), ("min_p", min_p, 0.0, lambda x: 0 <= x <= 1),
+  ):  # fmt: skip
+    each = isinstance(x, Tensor)
+    if not each and not ok(x):
+      raise ValueError(f"{name} is out of range: {x}")
+    rows.append(x if each else None)
+    numbers.append(off if each else x)
+  if is_compiling() or overridden(logits, uniform, *rows):
+    return sample_op(logits, uniform, *rows, *numbers)
+  return _native.sample(logits, uniform, *rows, *numbers)
