@@ -1,10 +1,10 @@
 """Attention of one new token per sequence over the paged cache, against the formula in 64 bits.
 
-Bounds, element by element: an output is a mean of values v_j with weights p_j.  Rounding the weights to the operands' type moves
-it by at most u * A, A = sum p_j |v_j|, u = 2^-9 (bfloat16), 2^-12 (float16), 0 (float32); logits that are off by e move it by at
-most 2 e A, e = (D + 8) 2^-23 * scale * max_j sum |q||k_j| for sums of D products in fp32 (plus cap * 2^-20 for the soft cap's
-tanh); the fp32 sums of weights and values by 2^-17 A at most; and rounding the result adds u |out| (2^-24 for float32),
-or half of the type's smallest step (2^-25 in float16) where that is more."""
+Bounds, element by element: an output is a mean of values v_j with weights p_j, A = sum p_j |v_j| >= |out|.  Logits that are off by e
+move it by at most 2 e A, e = (D + 8) 2^-23 * scale * max_j sum |q||k_j| for sums of D products in fp32 (plus cap * 2^-20 for the
+soft cap's tanh); the sums of weights and values, and weights as two 16-bit numbers, by 2^-17 A at most.  Rounding the result adds
+half a step, at most 2 u |out| <= u (|out| + A) with u = 2^-9 (bfloat16), 2^-12 (float16), u |out| with u = 2^-24 (float32), or half
+of the type's smallest step (2^-25 in float16) where that is more."""
 
 import math
 

@@ -3,13 +3,23 @@
 //   s_j = cap(scale * q . k_j),   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   m = max_j s_j
 //
 // in one pass over the keys, with a running maximum, sum and weighted sum of values (Milakov and Gimelshein, "Online normalizer
-// calculation for softmax", 2018).
+// calculation for softmax", 2018).  A key and its value are used by the g = Hq / Hkv query heads that share them: 2 g flops for
+// each element read, so it is the reading of the cache that bounds long calls, and the chain of dependent loads short ones.
+//
+// 16-bit and 8-bit caches (paged_attn_kernel): the g heads are the 16 columns of 16x16x32 matrix products (more than 16 heads: blocks
+// of 16, the unused columns zero), which costs a few percent of the time that the bytes take, whatever g is.  Layouts (lane: r = lane
+// % 16, g = lane / 16): A and B hold row / column r, k = 8 g + 0..7; C holds column r, rows 4 g + 0..3.  A wave takes 32 keys at a
+// time, straight from memory into the operands, without LDS and without an exchange between lanes:
+//   * scores are S^T = K Q^T, two products of 16 keys.  Row i of product t is key 8 (i / 4) + 4 t + i % 4, so that the scores of a
+//     lane, rows 4 g + 0..3 of both, are those of keys 8 g + 0..7, which is its share of the B operand of O^T += V^T P^T.
+//   * for V^T a lane needs 8 keys of one column, memory holds columns side by side: a lane loads the same DV / 16 columns of its 8
+//     keys, pairs the keys' halves with one v_perm per two elements, and product t takes column DV / 16 * r + t.  A row of values is
+//     read in one instruction by the 16 lanes of a group, and a lane ends with DV / 4 neighbouring columns of its head.
 #pragma once
+#include "attn_common.hpp"
 #include "kv_cache.hpp"
 
 namespace tp {
-
-constexpr float ATT_LOG2E = 1.4426950408889634f, ATT_LN2 = 0.6931471805599453f;
 
 struct PagedAttnArgs {
   PageRows k, v;
@@ -21,22 +31,23 @@ struct PagedAttnArgs {
   float* ws;
   int64_t q_b, q_h, o_b, o_h;
   int B, Hq, heads;  // heads: of keys and values
+  int blocks;        // of 16 query heads that share a kv head
+  int rows;          // query heads per block, at most 16
   float scale;       // log2(e) * sm_scale; without log2(e) where soft_cap is set
   float cap;         // soft_cap, 0: none
   int window;        // keys before the newest that are seen, negative: all
 };
 
 // ------------------------------------------------------------------------------------------------
-// one workgroup per (sequence, query head): a thread takes a key of every 256, then a few columns of the values
+// fp32: one workgroup per (sequence, query head): a thread takes a key of every 256, then a few columns of the values
 // ------------------------------------------------------------------------------------------------
 constexpr int PA_KEYS = 256;
-template <typename T, bool QUANT>
 __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs a) {
   __shared__ float q[512], p[PA_KEYS], part[4], acc_lds[PA_KEYS * 8];
   __shared__ int64_t at_v[PA_KEYS];
   const int b = blockIdx.x / a.Hq, h = blockIdx.x - b * a.Hq, kv = h / (a.Hq / a.heads), tid = threadIdx.x;
-  const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_b + h * a.q_h;
-  for (int i = tid; i < a.k.dim; i += PA_KEYS) q[i] = Elem<T>::to_f(qp[i]);
+  const float* qp = reinterpret_cast<const float*>(a.q) + b * a.q_b + h * a.q_h;
+  for (int i = tid; i < a.k.dim; i += PA_KEYS) q[i] = qp[i];
   const int n = min(a.lengths[b], a.table.width << a.table.page_shift);
   const int first = a.window >= 0 ? max(0, n - 1 - a.window) : 0;
   const int lane = tid & (a.v.group - 1), sub = tid / a.v.group, subs = PA_KEYS / a.v.group;
@@ -44,24 +55,18 @@ __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs 
   __syncthreads();
   for (int j0 = first; j0 < n; j0 += PA_KEYS) {
     const int j = j0 + tid, page = j < n ? a.table.page_of(b, j) : -1, slot = j & ((1 << a.table.page_shift) - 1);
-    float s = -INFINITY, vs = 1.f;
+    float s = -INFINITY;
     if (page >= 0) {
       const int64_t at = page * a.k.page + kv * a.k.head + slot * a.k.slot;
       s = 0.f;
       for (int d = 0; d < a.k.dim; d += 8) {
         float x[8];
-        if constexpr (QUANT) unpack_fp8(*reinterpret_cast<const u32x2*>(a.k.base + at + d), x);
-        else load_f<T, 8>(reinterpret_cast<const T*>(a.k.base) + at + d, x);
+        load_f<float, 8>(reinterpret_cast<const float*>(a.k.base) + at + d, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) s += x[e] * q[d + e];
       }
-      if constexpr (QUANT) {
-        const int64_t row = (((int64_t)page * a.heads + kv) << a.table.page_shift) + slot;
-        s *= a.k.scale[row];
-        vs = a.v.scale[row];
-      }
       s *= a.scale;
-      if (a.cap > 0.f) s = a.cap * ATT_LOG2E * tanhf(s / a.cap);
+      if (a.cap > 0.f) s = a.cap * LOG2E * tanhf(s / a.cap);
     }
     float mx = wave_max(s);
     if ((tid & 63) == 0) part[tid >> 6] = mx;
@@ -71,7 +76,7 @@ __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs 
     const float shrink = exp2f(m - base);
     const float w = page >= 0 ? exp2f(s - base) : 0.f;
     l = l * shrink + w;  // this thread's keys
-    p[tid] = w * vs;
+    p[tid] = w;
     at_v[tid] = page >= 0 ? page * a.v.page + kv * a.v.head + slot * a.v.slot : -1;
     m = m_new;
     __syncthreads();
@@ -81,8 +86,7 @@ __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs 
       for (int i = sub; i < PA_KEYS && j0 + i < n; i += subs) {
         if (at_v[i] < 0) continue;  // (not loaded: what lies there takes no part, whatever it is)
         float x[8];
-        if constexpr (QUANT) unpack_fp8(*reinterpret_cast<const u32x2*>(a.v.base + at_v[i] + lane * 8), x);
-        else load_f<T, 8>(reinterpret_cast<const T*>(a.v.base) + at_v[i] + lane * 8, x);
+        load_f<float, 8>(reinterpret_cast<const float*>(a.v.base) + at_v[i] + lane * 8, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) acc[e] += p[i] * x[e];
       }
@@ -98,14 +102,433 @@ __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs 
   for (int d = tid; d < a.v.dim; d += PA_KEYS) {
     float o = 0.f;
     for (int i = 0; i < subs; i++) o += acc_lds[(i * a.v.group + d / 8) * 8 + d % 8];
-    reinterpret_cast<T*>(a.out)[b * a.o_b + h * a.o_h + d] = Elem<T>::from_f(l != 0.f ? o / l : 0.f);
+    reinterpret_cast<float*>(a.out)[b * a.o_b + h * a.o_h + d] = l != 0.f ? o / l : 0.f;
   }
-  if (tid == 0 && a.lse) a.lse[(int64_t)b * a.Hq + h] = l != 0.f ? (m + log2f(l)) * ATT_LN2 : -INFINITY;
+  if (tid == 0 && a.lse) a.lse[(int64_t)b * a.Hq + h] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+}
+
+// ------------------------------------------------------------------------------------------------
+// how the work is shared out
+// ------------------------------------------------------------------------------------------------
+// A segment is a (sequence, kv head, block of query heads); a unit is what a workgroup takes of it in one step, 32 keys a wave.
+// Segments in order are one line of units, of which every workgroup takes the same number: a long sequence among short ones is
+// shared by many workgroups, and short ones go several to a workgroup.  Nothing of that needs the host to know the lengths.  A
+// segment that lies in one workgroup leaves as the result; one that is cut leaves its pieces (maximum, sum, weighted sum) in the
+// workspace: piece 2 w of workgroup w if it begins there with the workgroup, else 2 w + 1; paged_attn_join_kernel adds them up in
+// their order, so that a call gives the same bits every time.
+constexpr int PA_WAVES = 8, PA_TILE = 32, PA_UNIT = PA_WAVES * PA_TILE;
+
+struct Keys {  // of one sequence: [first, end), and `base`, the multiple of 32 at or below first, where units begin
+  int first, end, base, units;
+  __device__ __forceinline__ Keys(const PagedAttnArgs& a, int b) {
+    end = max(0, min(a.lengths[b], a.table.width << a.table.page_shift));
+    first = a.window >= 0 ? max(0, end - 1 - a.window) : 0;
+    base = first & ~(PA_TILE - 1);
+    units = max(1, (end - base + PA_UNIT - 1) / PA_UNIT);  // (an empty sequence has its unit, too: its zeros have to be written)
+  }
+};
+
+struct Share {
+  int per;      // units per workgroup
+  int total;    // units
+  int b, at;    // the sequence that unit `u` belongs to, and the number of units before that sequence
+};
+// Every wave works this out by itself; a lane counts ceil(B / 64) sequences.
+__device__ __forceinline__ int lane_units(const PagedAttnArgs& a, int b0, int b1) {
+  int n = 0;
+  for (int b = b0; b < b1; b++) n += Keys(a, b).units;
+  return n;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+__device__ __forceinline__ Share share_of(const PagedAttnArgs& a, int groups, int least, int w) {
+  const int lane = threadIdx.x & 63, each = (a.B + 63) / 64, segs = a.heads * a.blocks;
+  const int b0 = min(lane * each, a.B), b1 = min(b0 + each, a.B);
+  const int n = lane_units(a, b0, b1), upto = wave_scan(n, lane);
+  Share s;
+  s.total = __shfl(upto, 63, 64) * segs;
+  s.per = max(least, (s.total + groups - 1) / groups);
+  const int u = w * s.per;
+  s.b = s.at = 0;
+  if (u >= s.total) return s;
+  const uint64_t past = __ballot(upto * segs > u);
+  const int l0 = __ffsll((unsigned long long)past) - 1;
+  s.b = min(l0 * each, a.B - 1);
+  s.at = __shfl(upto - n, l0, 64) * segs;
+  for (;;) {  // (ends within the lane's sequences: their units reach beyond u)
+    const int here = Keys(a, s.b).units * segs;
+    if (s.at + here > u) break;
+    s.at += here;
+    s.b++;
+  }
+  return s;
+}
+
+constexpr int pa_piece_floats(int dv) { return 2 * 16 + 16 * dv; }  // maxima, sums, weighted sums
+
+template <typename T> struct MM;
+template <> struct MM<bf16_t> {
+  static __device__ __forceinline__ f32x4 dot(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ unsigned from_fp8(unsigned w, bool hi) {
+    return __builtin_bit_cast(unsigned, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+  }
+};
+template <> struct MM<f16_t> {
+  static __device__ __forceinline__ f32x4 dot(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ unsigned from_fp8(unsigned w, bool hi) {
+    return __builtin_bit_cast(unsigned, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+  }
+};
+
+// over the four lane groups that hold one head
+__device__ __forceinline__ float groups_max(float v) {
+  v = half_max(v);
+  return fmaxf(v, __shfl_xor(v, 16, 64));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  v = half_sum(v);
+  return v + __shfl_xor(v, 16, 64);
+}
+
+// What a wave has of a segment.  The maximum m is lazy: it moves only when a score exceeds it by more than 8 (log2 units), so that the
+// sums are rarely rescaled.  Weights (at most 2^8) go into the product as two numbers of type T, the rounded weight and the rest, so
+// that nothing but the result is rounded to 16 bits; the second product costs less than the bytes leave room for.  In an 8-bit cache
+// they carry the value's scale, and for float16, whose range is short, relative to 2^c, c the largest exponent of a scale so far.
+template <int DV> struct Partial {
+  float m, l;  // of this lane's head; l over this lane's keys
+  int c;
+  f32x4 o[DV / 16];
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+    c = -150;
+#pragma unroll
+    for (int t = 0; t < DV / 16; t++) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+};
+
+template <typename T, bool QUANT, int DQK, int DV>
+struct PagedTile {
+  typedef T v8 __attribute__((ext_vector_type(8)));
+  static constexpr int KS = DQK / 32;                 // products per 16 keys
+  static constexpr int KL = QUANT ? DQK / 64 : KS;    // 16-byte loads of a key per lane
+  static constexpr int C = DV / 16;                   // columns of V per lane
+  static constexpr int VB = C * (QUANT ? 1 : 2);      // their bytes
+  static constexpr bool RANGE = QUANT && std::is_same<T, f16_t>::value;
+
+  static __device__ __forceinline__ void load_q(const PagedAttnArgs& a, const T* q, bool mine, v8 (&f)[KS]) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < KS; i++) {
+      // (8-bit keys: 16 bytes of a key, two products' shares, lie side by side)
+      const int d = QUANT ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+      f[i] = mine ? *reinterpret_cast<const v8*>(q + d) : v8{};
+    }
+  }
+
+  // keys key0 .. key0 + 31 of sequence b, those in [first, end)
+  static __device__ __forceinline__ void run(const PagedAttnArgs& a, const v8 (&q)[KS], int b, int kv, int key0, int first, int end, Partial<DV>& p) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, mask = (1 << a.table.page_shift) - 1;
+    const int tk = key0 + 8 * (r >> 2), tv = key0 + 8 * g;  // eight keys from a multiple of 8 lie in one page
+    const int pk = tk < end ? a.table.page_of(b, tk) : -1, pv = tv < end ? a.table.page_of(b, tv) : -1;
+    constexpr int E = QUANT ? 1 : 2;
+    const char* kp = a.k.base + E * (max(pk, 0) * a.k.page + kv * a.k.head + ((tk & mask) + (r & 3)) * a.k.slot) + 16 * g;
+    const char* vp = a.v.base + E * (max(pv, 0) * a.v.page + kv * a.v.head + (tv & mask) * a.v.slot) + VB * r;
+    u32x4 kr[2][KL];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int i = 0; i < KL; i++) kr[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + E * 4 * t * a.k.slot + 64 * i));
+    unsigned vr[8][VB / 4];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      typedef unsigned row_t __attribute__((ext_vector_type(VB / 4)));
+      if constexpr (VB == 4) {
+        vr[e][0] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(vp + E * e * a.v.slot));
+      } else {
+        const row_t x = __builtin_nontemporal_load(reinterpret_cast<const row_t*>(vp + E * e * a.v.slot));
+#pragma unroll
+        for (int i = 0; i < VB / 4; i++) vr[e][i] = x[i];
+      }
+    }
+    float ks[8], vs[8];
+    if constexpr (QUANT) {
+      const int64_t at = (((int64_t)max(pv, 0) * a.heads + kv) << a.table.page_shift) + (tv & mask);
+      load_f<float, 8>(a.k.scale + at, ks);
+      load_f<float, 8>(a.v.scale + at, vs);
+    }
+    // scores
+    float s[8];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KS; i++) {
+        u32x4 f;
+        if constexpr (QUANT) {
+#pragma unroll
+          for (int w = 0; w < 4; w++) f[w] = MM<T>::from_fp8(kr[t][i / 2][2 * (i % 2) + w / 2], w % 2);
+        } else {
+          f = kr[t][i];
+        }
+        acc = MM<T>::dot(__builtin_bit_cast(v8, f), q[i], acc);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if constexpr (QUANT) s[e] *= ks[e];
+      s[e] *= a.scale;
+    }
+    if (a.cap > 0.f) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) s[e] = a.cap * LOG2E * fast_tanh(s[e] / a.cap);
+    }
+    const bool whole = pv >= 0 && tv >= first && tv + 8 <= end;
+    if (!__all(whole)) {
+      // what lies in slots without a key takes no part, whatever it is: no score, and zeros for the products
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const bool in = pv >= 0 && tv + e >= first && tv + e < end;
+        s[e] = in ? s[e] : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VB / 4; i++) vr[e][i] = in ? vr[e][i] : 0u;
+        if constexpr (QUANT) vs[e] = in ? vs[e] : 0.f;
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[e]);
+    mx = groups_max(mx);
+    int cx = p.c;
+    if constexpr (RANGE) {
+      float top = vs[0];
+#pragma unroll
+      for (int e = 1; e < 8; e++) top = fmaxf(top, vs[e]);
+      top = groups_max(top);  // (the same in every lane)
+      if (top > 0.f) cx = max(cx, __builtin_amdgcn_frexp_expf(top));
+    }
+    if (__any(mx > p.m + 8.f || (mx > -INFINITY && p.m == -INFINITY)) || (RANGE && cx > p.c)) {
+      const float m = fmaxf(p.m, mx), shrink = m == -INFINITY ? 1.f : fast_exp2(p.m - m);
+      const float so = RANGE ? __builtin_amdgcn_ldexpf(shrink, p.c - cx) : shrink;
+      p.l *= shrink;
+#pragma unroll
+      for (int t = 0; t < C; t++) p.o[t] *= so;
+      p.m = m;
+      p.c = cx;
+    }
+    const float m = p.m == -INFINITY ? 0.f : p.m;
+    v8 w, rest;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      float x = fast_exp2(s[e] - m);
+      p.l += x;
+      if constexpr (RANGE) x *= __builtin_amdgcn_ldexpf(vs[e], -p.c);
+      else if constexpr (QUANT) x *= vs[e];
+      w[e] = (T)x;
+      rest[e] = (T)(x - (float)w[e]);
+    }
+    // values: column C r + t of the eight keys, paired from the rows as they came
+    unsigned cols[8][C / 2];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int i = 0; i < C / 2; i++) {
+        if constexpr (QUANT) cols[e][i] = MM<T>::from_fp8(vr[e][i / 2], i % 2);
+        else cols[e][i] = vr[e][i];
+      }
+#pragma unroll
+    for (int t = 0; t < C; t++) {
+      u32x4 f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) f[i] = __builtin_amdgcn_perm(cols[2 * i + 1][t / 2], cols[2 * i][t / 2], t % 2 ? 0x07060302u : 0x05040100u);
+      p.o[t] = MM<T>::dot(__builtin_bit_cast(v8, f), w, p.o[t]);
+      p.o[t] = MM<T>::dot(__builtin_bit_cast(v8, f), rest, p.o[t]);
+    }
+  }
+};
+
+// One segment's sums over the waves (or pieces) that hold a part of it.  `n` parts: m, l at parts[i * stride + row], [.. + 16 + row],
+// weighted sums at [.. + 32 + row * ROW + d].  Threads take four columns each.
+template <typename T, int DV, int ROW>
+__device__ __forceinline__ void join_parts(const PagedAttnArgs& a, int b, int h0, int rows, const float* parts, int64_t stride, int n, int threads, bool result,
+                                           float* piece) {
+  for (int i = threadIdx.x; i < rows * (DV / 4); i += threads) {
+    const int row = i / (DV / 4), d = (i - row * (DV / 4)) * 4;
+    float m = -INFINITY;
+    for (int k = 0; k < n; k++) m = fmaxf(m, parts[k * stride + row]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < n; k++) {
+      const float* p = parts + k * stride;
+      const float f = fast_exp2(p[row] - base);
+      l += f * p[16 + row];
+      o += f * *reinterpret_cast<const f32x4*>(p + 32 + row * ROW + d);
+    }
+    if (result) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(a.out) + b * a.o_b + (h0 + row) * a.o_h + d) = pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      if (d == 0 && a.lse) a.lse[(int64_t)b * a.Hq + h0 + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+    } else {
+      *reinterpret_cast<f32x4*>(piece + 32 + row * DV + d) = o;
+      if (d == 0) {
+        piece[row] = m;
+        piece[16 + row] = l;
+      }
+    }
+  }
+}
+
+// WHOLE: a workgroup per segment (few keys at most); otherwise equal shares of all units
+template <typename T, bool QUANT, int DQK, int DV, bool WHOLE>
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_attn_kernel(PagedAttnArgs a, int least) {
+  typedef PagedTile<T, QUANT, DQK, DV> Tile;
+  constexpr int ROW = DV + 4;  // (heads 4 banks apart)
+  extern __shared__ float lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int segs = a.heads * a.blocks, rep = a.Hq / a.heads;
+  int u, u1, b, at;
+  if constexpr (WHOLE) {
+    b = blockIdx.x / segs;
+    at = 0;  // (units are counted from the sequence's first)
+  } else {
+    const Share s = share_of(a, gridDim.x, least, blockIdx.x);
+    u = blockIdx.x * s.per;
+    u1 = min(u + s.per, s.total);
+    if (u >= u1) return;
+    b = s.b;
+    at = s.at;
+  }
+  Keys keys(a, b);
+  if constexpr (WHOLE) {
+    u = (blockIdx.x - b * segs) * keys.units;
+    u1 = u + keys.units;
+  }
+  const int stride = 32 + a.rows * ROW;
+  float* mine = lds + wave * stride;
+  int piece = 2 * blockIdx.x;
+  while (u < u1) {
+    const int seg = (u - at) / keys.units, step0 = u - at - seg * keys.units, step1 = min(keys.units, step0 + u1 - u);
+    const int kv = seg / a.blocks, block = seg - kv * a.blocks, h0 = kv * rep + 16 * block, rows = min(16, rep - 16 * block);
+    typename Tile::v8 q[Tile::KS];
+    Tile::load_q(a, reinterpret_cast<const T*>(a.q) + b * a.q_b + (h0 + r) * a.q_h, r < rows, q);
+    Partial<DV> p;
+    p.clear();
+    for (int step = step0; step < step1; step++) {
+      const int key0 = keys.base + (step * PA_WAVES + wave) * PA_TILE;
+      if (key0 < keys.end) Tile::run(a, q, b, kv, key0, keys.first, keys.end, p);
+    }
+    p.l = groups_sum(p.l);
+    if (r < rows) {
+      if (g == 0) {
+        mine[r] = p.m;
+        mine[16 + r] = p.l;
+      }
+      float* o = mine + 32 + r * ROW + (DV / 4) * g;
+      const float up = Tile::RANGE ? __builtin_amdgcn_ldexpf(1.f, p.c) : 1.f;
+      constexpr int C = DV / 16;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int t = 0; t < C; t += 4) {
+          f32x4 x{p.o[t][e], p.o[t + 1][e], p.o[t + 2][e], p.o[t + 3][e]};
+          *reinterpret_cast<f32x4*>(o + e * C + t) = x * up;
+        }
+    }
+    __syncthreads();
+    const bool result = step0 == 0 && step1 == keys.units;
+    join_parts<T, DV, ROW>(a, b, h0, rows, lds, stride, PA_WAVES, 64 * PA_WAVES, result, a.ws + (int64_t)piece * pa_piece_floats(DV));
+    piece = 2 * blockIdx.x + 1;
+    u += step1 - step0;
+    if (u < u1) {
+      __syncthreads();
+      if (u - at == keys.units * segs) {
+        at = u;
+        keys = Keys(a, ++b);
+      }
+    }
+  }
+}
+
+// Workgroup w looks at the first unit of share w + 1: where that is inside a segment whose first cut it is, it adds the segment up.
+constexpr int PA_JOIN = 256;
+template <typename T, int DV>
+__global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs a, int groups, int least) {
+  const int rep = a.Hq / a.heads, w = blockIdx.x + 1;
+  const Share s = share_of(a, groups, least, w);
+  const int u = w * s.per;
+  if (u >= s.total) return;
+  const Keys keys(a, s.b);
+  const int seg = (u - s.at) / keys.units, begin = s.at + seg * keys.units, end = begin + keys.units;
+  if (begin == u || begin < u - s.per) return;  // no cut, or not its first
+  const int first = begin / s.per, last = (end - 1) / s.per;  // (workgroups)
+  const int kv = seg / a.blocks, block = seg - kv * a.blocks, h0 = kv * rep + 16 * block, rows = min(16, rep - 16 * block);
+  // its pieces: the first workgroup's last one, then the others' first ones
+  const int64_t one = pa_piece_floats(DV);
+  const float* p0 = a.ws + (2 * first + (first * s.per == begin ? 0 : 1)) * one;
+  for (int i = threadIdx.x; i < rows * (DV / 4); i += PA_JOIN) {
+    const int row = i / (DV / 4), d = (i - row * (DV / 4)) * 4;
+    float m = p0[row];
+    for (int k = first + 1; k <= last; k++) m = fmaxf(m, a.ws[2 * k * one + row]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float f = fast_exp2(p0[row] - base), l = f * p0[16 + row];
+    f32x4 o = f * *reinterpret_cast<const f32x4*>(p0 + 32 + row * DV + d);
+    for (int k = first + 1; k <= last; k++) {
+      const float* p = a.ws + 2 * k * one;
+      f = fast_exp2(p[row] - base);
+      l += f * p[16 + row];
+      o += f * *reinterpret_cast<const f32x4*>(p + 32 + row * DV + d);
+    }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+    *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(a.out) + s.b * a.o_b + (h0 + row) * a.o_h + d) = pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (d == 0 && a.lse) a.lse[(int64_t)s.b * a.Hq + h0 + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------
+// Workgroups of a call and the least units each takes.  Where the table has room for no more than `WHOLE_UNITS` units a sequence, a
+// workgroup takes a whole segment, no piece is left over and no second launch follows.
+struct PagedPlan {
+  bool whole;
+  int groups, least;
+};
+constexpr int PA_GROUPS = 512, PA_LEAST = 2, PA_WHOLE_UNITS = 2;
+inline PagedPlan paged_plan(const tp_kv_cache* c, int B, int Hq) {
+  const int64_t segs = (int64_t)B * c->heads * ((Hq / c->heads + 15) / 16);
+  const int64_t units = ((int64_t)c->table_width * c->page_size + PA_TILE + PA_UNIT - 1) / PA_UNIT;
+  if (units <= PA_WHOLE_UNITS) return {true, (int)segs, 1};
+  return {false, (int)std::min<int64_t>(PA_GROUPS, (segs * units + PA_LEAST - 1) / PA_LEAST), PA_LEAST};
+}
+
+template <typename T, bool QUANT, int DQK, int DV>
+int paged_launch(const PagedAttnArgs& a, const PagedPlan& plan, hipStream_t st) {
+  const int lds = PA_WAVES * (32 + a.rows * (DV + 4)) * 4;
+  const auto kern = plan.whole ? paged_attn_kernel<T, QUANT, DQK, DV, true> : paged_attn_kernel<T, QUANT, DQK, DV, false>;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    TP_REQUIRE(e == hipSuccess, TP_ERR_LAUNCH, "tp_paged_attn: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+  }
+  kern<<<plan.groups, 64 * PA_WAVES, lds, st>>>(a, plan.least);
+  if (!plan.whole && plan.groups > 1) paged_attn_join_kernel<T, DV><<<plan.groups - 1, PA_JOIN, 0, st>>>(a, plan.groups, plan.least);
+  return check_launch("tp_paged_attn");
 }
 
 }  // namespace tp
 
-extern "C" size_t tp_paged_attn_workspace_bytes(const tp_kv_cache* c, int B, int Hq, int dtype) { return 0; }
+extern "C" size_t tp_paged_attn_workspace_bytes(const tp_kv_cache* c, int B, int Hq, int dtype) {
+  using namespace tp;
+  if (check_cache(c, dtype, B, "tp_paged_attn_workspace_bytes") || Hq < 1 || Hq % c->heads || dtype == TP_F32) return 0;
+  const PagedPlan plan = paged_plan(c, B, Hq);
+  return plan.whole ? 0 : sizeof(float) * 2 * plan.groups * pa_piece_floats(c->v_dim);
+}
 
 extern "C" int tp_paged_attn(const tp_kv_cache* c, const void* q, const int32_t* lengths, void* out, float* lse, void* ws, int B, int Hq,
                              const int64_t* q_strides, const int64_t* o_strides, float sm_scale, int window_left, float soft_cap, int dtype,
@@ -122,10 +545,26 @@ extern "C" int tp_paged_attn(const tp_kv_cache* c, const void* q, const int32_t*
   for (int i = 0; i < 2; i++)
     TP_REQUIRE(q_strides[i] * e % 16 == 0 && o_strides[i] * e % 16 == 0, TP_ERR_BAD_ARG, "tp_paged_attn: strides must keep rows 16-byte aligned");
   TP_REQUIRE((int64_t)B * Hq < (1ll << 24), TP_ERR_UNSUPPORTED, "tp_paged_attn: too many rows");
-  PagedAttnArgs a{rows_of(c, false), rows_of(c, true), table_of(c), q, lengths, out, lse, (float*)ws, q_strides[0], q_strides[1], o_strides[0],
-                  o_strides[1], B, Hq, c->heads, soft_cap > 0.f ? sm_scale : sm_scale * ATT_LOG2E, soft_cap, window_left};
+  TP_REQUIRE((int64_t)B * c->heads * ((Hq / c->heads + 15) / 16) * (((int64_t)c->table_width * c->page_size) / PA_UNIT + 2) < (1ll << 31) - PA_GROUPS,
+             TP_ERR_UNSUPPORTED, "tp_paged_attn: the table covers too many keys");
+  const int rep = Hq / c->heads;
+  const PagedAttnArgs a{rows_of(c, false), rows_of(c, true), table_of(c), q, lengths, out, lse, (float*)ws, q_strides[0], q_strides[1], o_strides[0],
+                        o_strides[1], B, Hq, c->heads, (rep + 15) / 16, std::min(rep, 16), soft_cap > 0.f ? sm_scale : sm_scale * LOG2E, soft_cap,
+                        window_left};
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == TP_F32) {
+    paged_attn_rows_kernel<<<B * Hq, PA_KEYS, 0, st>>>(a);
+    return check_launch("tp_paged_attn");
+  }
+  const PagedPlan plan = paged_plan(c, B, Hq);
+  TP_REQUIRE(plan.whole || (ws && aligned16(ws)), TP_ERR_BAD_ARG, "tp_paged_attn: the workspace must be there and start at a 16-byte address");
+  int rc = TP_OK;
   kv_dispatch(dtype, c->dtype == TP_FP8, [&](auto t, auto quant) {
-    paged_attn_rows_kernel<decltype(t), quant.value><<<B * Hq, PA_KEYS, 0, (hipStream_t)stream>>>(a);
+    typedef decltype(t) T;
+    if constexpr (!std::is_same<T, float>::value) {
+      constexpr bool Q = quant.value;
+      rc = c->k_dim == 64 ? paged_launch<T, Q, 64, 64>(a, plan, st) : c->k_dim == 128 ? paged_launch<T, Q, 128, 128>(a, plan, st) : paged_launch<T, Q, 192, 128>(a, plan, st);
+    }
   });
-  return check_launch("tp_paged_attn");
+  return rc;
 }
