@@ -116,29 +116,24 @@ __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs 
 // segment that lies in one workgroup leaves as the result; one that is cut leaves its pieces (maximum, sum, weighted sum) in the
 // workspace: piece 2 w of workgroup w if it begins there with the workgroup, else 2 w + 1; paged_attn_join_kernel adds them up in
 // their order, so that a call gives the same bits every time.
-constexpr int PA_WAVES = 8, PA_TILE = 32, PA_UNIT = PA_WAVES * PA_TILE;
+constexpr int PA_TILE = 32;
 
 struct Keys {  // of one sequence: [first, end), and `base`, the multiple of 32 at or below first, where units begin
-  int first, end, base, units;
-  __device__ __forceinline__ Keys(const PagedAttnArgs& a, int b) {
-    end = max(0, min(a.lengths[b], a.table.width << a.table.page_shift));
+  int first, end, base;
+  __device__ __forceinline__ Keys(const PagedAttnArgs& a, int length) {
+    end = max(0, min(length, a.table.width << a.table.page_shift));
     first = a.window >= 0 ? max(0, end - 1 - a.window) : 0;
     base = first & ~(PA_TILE - 1);
-    units = max(1, (end - base + PA_UNIT - 1) / PA_UNIT);  // (an empty sequence has its unit, too: its zeros have to be written)
   }
+  // (an empty sequence has its unit, too: its zeros have to be written)
+  __device__ __forceinline__ int units(int unit) const { return max(1, (end - base + unit - 1) / unit); }
 };
 
 struct Share {
-  int per;      // units per workgroup
-  int total;    // units
-  int b, at;    // the sequence that unit `u` belongs to, and the number of units before that sequence
+  int per, total;  // units per workgroup, and in all
+  int b, at;       // the sequence that the share's first unit belongs to, and the number of units before that sequence
+  int length;      // that sequence's
 };
-// Every wave works this out by itself; a lane counts ceil(B / 64) sequences.
-__device__ __forceinline__ int lane_units(const PagedAttnArgs& a, int b0, int b1) {
-  int n = 0;
-  for (int b = b0; b < b1; b++) n += Keys(a, b).units;
-  return n;
-}
 __device__ __forceinline__ int wave_scan(int v, int lane) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -147,30 +142,48 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
   }
   return v;
 }
+// Every wave works this out by itself; a lane counts ceil(B / 64) sequences.
+template <int UNIT>
 __device__ __forceinline__ Share share_of(const PagedAttnArgs& a, int groups, int least, int w) {
   const int lane = threadIdx.x & 63, each = (a.B + 63) / 64, segs = a.heads * a.blocks;
   const int b0 = min(lane * each, a.B), b1 = min(b0 + each, a.B);
-  const int n = lane_units(a, b0, b1), upto = wave_scan(n, lane);
+  int n = 0, length = 0;
+  for (int b = b0; b < b1; b++) {
+    length = a.lengths[b];
+    n += Keys(a, length).units(UNIT);
+  }
+  const int upto = wave_scan(n, lane);
   Share s;
   s.total = __shfl(upto, 63, 64) * segs;
   s.per = max(least, (s.total + groups - 1) / groups);
   const int u = w * s.per;
-  s.b = s.at = 0;
+  s.b = s.at = s.length = 0;
   if (u >= s.total) return s;
-  const uint64_t past = __ballot(upto * segs > u);
-  const int l0 = __ffsll((unsigned long long)past) - 1;
+  const int l0 = __ffsll((unsigned long long)__ballot(upto * segs > u)) - 1;
   s.b = min(l0 * each, a.B - 1);
   s.at = __shfl(upto - n, l0, 64) * segs;
-  for (;;) {  // (ends within the lane's sequences: their units reach beyond u)
-    const int here = Keys(a, s.b).units * segs;
-    if (s.at + here > u) break;
-    s.at += here;
-    s.b++;
+  s.length = __shfl(length, l0, 64);
+  if (each > 1) {
+    for (;;) {  // (ends within the lane's sequences: their units reach beyond u)
+      s.length = a.lengths[s.b];
+      const int here = Keys(a, s.length).units(UNIT) * segs;
+      if (s.at + here > u) break;
+      s.at += here;
+      s.b++;
+    }
   }
   return s;
 }
 
+// What a workgroup whose first unit lies inside a segment says about it, where this is the segment's first cut (else rows = 0)
+struct SegmentCut {
+  int rows, b, h0, first, last, lead;  // its workgroups; 1 where the first one's piece is not its first
+  int none[2];
+};
 constexpr int pa_piece_floats(int dv) { return 2 * 16 + 16 * dv; }  // maxima, sums, weighted sums
+__device__ __forceinline__ float* pa_piece(const PagedAttnArgs& a, int groups, int i, int dv) {  // behind the cuts
+  return a.ws + (int64_t)groups * (int)(sizeof(SegmentCut) / 4) + (int64_t)i * pa_piece_floats(dv);
+}
 
 template <typename T> struct MM;
 template <> struct MM<bf16_t> {
@@ -232,37 +245,56 @@ struct PagedTile {
     }
   }
 
-  // keys key0 .. key0 + 31 of sequence b, those in [first, end)
-  static __device__ __forceinline__ void run(const PagedAttnArgs& a, const v8 (&q)[KS], int b, int kv, int key0, int first, int end, Partial<DV>& p) {
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, mask = (1 << a.table.page_shift) - 1;
+  // One tile of keys key0 .. key0 + 31 on its way: where it lies, then what was loaded.
+  struct Where {
+    int pk, pv;  // pages of this lane's rows of keys and of values, -1: none
+  };
+  struct Data {
+    u32x4 k[2][KL];
+    unsigned v[8][VB / 4];
+    float ks[QUANT ? 8 : 1], vs[QUANT ? 8 : 1];
+    int tv;     // the first of this lane's eight keys
+    bool page;  // they lie in a page
+  };
+  static __device__ __forceinline__ Where find(const PagedAttnArgs& a, int b, int key0) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int tk = key0 + 8 * (r >> 2), tv = key0 + 8 * g;  // eight keys from a multiple of 8 lie in one page
-    const int pk = tk < end ? a.table.page_of(b, tk) : -1, pv = tv < end ? a.table.page_of(b, tv) : -1;
+    return {a.table.page_of(b, tk), a.table.page_of(b, tv)};
+  }
+  // (Rows without a page are read from page 0, which is there, and dropped later.)
+  static __device__ __forceinline__ void load(const PagedAttnArgs& a, const Where& at, int kv, int key0, Data& x) {
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, mask = (1 << a.table.page_shift) - 1;
+    const int tk = key0 + 8 * (r >> 2), tv = key0 + 8 * g;
     constexpr int E = QUANT ? 1 : 2;
-    const char* kp = a.k.base + E * (max(pk, 0) * a.k.page + kv * a.k.head + ((tk & mask) + (r & 3)) * a.k.slot) + 16 * g;
-    const char* vp = a.v.base + E * (max(pv, 0) * a.v.page + kv * a.v.head + (tv & mask) * a.v.slot) + VB * r;
-    u32x4 kr[2][KL];
+    const char* kp = a.k.base + E * (max(at.pk, 0) * a.k.page + kv * a.k.head + ((tk & mask) + (r & 3)) * a.k.slot) + 16 * g;
+    const char* vp = a.v.base + E * (max(at.pv, 0) * a.v.page + kv * a.v.head + (tv & mask) * a.v.slot) + VB * r;
+    if constexpr (QUANT) {
+      const int64_t row = (((int64_t)max(at.pv, 0) * a.heads + kv) << a.table.page_shift) + (tv & mask);
+      load_f<float, 8>(a.k.scale + row, x.ks);
+      load_f<float, 8>(a.v.scale + row, x.vs);
+    }
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int i = 0; i < KL; i++) kr[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + E * 4 * t * a.k.slot + 64 * i));
-    unsigned vr[8][VB / 4];
+      for (int i = 0; i < KL; i++) x.k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + E * 4 * t * a.k.slot + 64 * i));
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       typedef unsigned row_t __attribute__((ext_vector_type(VB / 4)));
       if constexpr (VB == 4) {
-        vr[e][0] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(vp + E * e * a.v.slot));
+        x.v[e][0] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(vp + E * e * a.v.slot));
       } else {
-        const row_t x = __builtin_nontemporal_load(reinterpret_cast<const row_t*>(vp + E * e * a.v.slot));
+        const row_t w = __builtin_nontemporal_load(reinterpret_cast<const row_t*>(vp + E * e * a.v.slot));
 #pragma unroll
-        for (int i = 0; i < VB / 4; i++) vr[e][i] = x[i];
+        for (int i = 0; i < VB / 4; i++) x.v[e][i] = w[i];
       }
     }
-    float ks[8], vs[8];
-    if constexpr (QUANT) {
-      const int64_t at = (((int64_t)max(pv, 0) * a.heads + kv) << a.table.page_shift) + (tv & mask);
-      load_f<float, 8>(a.k.scale + at, ks);
-      load_f<float, 8>(a.v.scale + at, vs);
-    }
+    x.tv = tv;
+    x.page = at.pv >= 0;
+  }
+
+  // takes the keys of a tile that are in [first, end) into the sums
+  static __device__ __forceinline__ void add(const PagedAttnArgs& a, const v8 (&q)[KS], Data& x, int first, int end, Partial<DV>& p) {
+    const int tv = x.tv;
     // scores
     float s[8];
 #pragma unroll
@@ -273,9 +305,9 @@ struct PagedTile {
         u32x4 f;
         if constexpr (QUANT) {
 #pragma unroll
-          for (int w = 0; w < 4; w++) f[w] = MM<T>::from_fp8(kr[t][i / 2][2 * (i % 2) + w / 2], w % 2);
+          for (int w = 0; w < 4; w++) f[w] = MM<T>::from_fp8(x.k[t][i / 2][2 * (i % 2) + w / 2], w % 2);
         } else {
-          f = kr[t][i];
+          f = x.k[t][i];
         }
         acc = MM<T>::dot(__builtin_bit_cast(v8, f), q[i], acc);
       }
@@ -284,23 +316,23 @@ struct PagedTile {
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      if constexpr (QUANT) s[e] *= ks[e];
+      if constexpr (QUANT) s[e] *= x.ks[e];
       s[e] *= a.scale;
     }
     if (a.cap > 0.f) {
 #pragma unroll
       for (int e = 0; e < 8; e++) s[e] = a.cap * LOG2E * fast_tanh(s[e] / a.cap);
     }
-    const bool whole = pv >= 0 && tv >= first && tv + 8 <= end;
+    const bool whole = x.page && tv >= first && tv + 8 <= end;
     if (!__all(whole)) {
       // what lies in slots without a key takes no part, whatever it is: no score, and zeros for the products
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const bool in = pv >= 0 && tv + e >= first && tv + e < end;
+        const bool in = x.page && tv + e >= first && tv + e < end;
         s[e] = in ? s[e] : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < VB / 4; i++) vr[e][i] = in ? vr[e][i] : 0u;
-        if constexpr (QUANT) vs[e] = in ? vs[e] : 0.f;
+        for (int i = 0; i < VB / 4; i++) x.v[e][i] = in ? x.v[e][i] : 0u;
+        if constexpr (QUANT) x.vs[e] = in ? x.vs[e] : 0.f;
       }
     }
     float mx = s[0];
@@ -309,9 +341,9 @@ struct PagedTile {
     mx = groups_max(mx);
     int cx = p.c;
     if constexpr (RANGE) {
-      float top = vs[0];
+      float top = x.vs[0];
 #pragma unroll
-      for (int e = 1; e < 8; e++) top = fmaxf(top, vs[e]);
+      for (int e = 1; e < 8; e++) top = fmaxf(top, x.vs[e]);
       top = groups_max(top);  // (the same in every lane)
       if (top > 0.f) cx = max(cx, __builtin_amdgcn_frexp_expf(top));
     }
@@ -328,12 +360,12 @@ struct PagedTile {
     v8 w, rest;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      float x = fast_exp2(s[e] - m);
-      p.l += x;
-      if constexpr (RANGE) x *= __builtin_amdgcn_ldexpf(vs[e], -p.c);
-      else if constexpr (QUANT) x *= vs[e];
-      w[e] = (T)x;
-      rest[e] = (T)(x - (float)w[e]);
+      float y = fast_exp2(s[e] - m);
+      p.l += y;
+      if constexpr (RANGE) y *= __builtin_amdgcn_ldexpf(x.vs[e], -p.c);
+      else if constexpr (QUANT) y *= x.vs[e];
+      w[e] = (T)y;
+      rest[e] = (T)(y - (float)w[e]);
     }
     // values: column C r + t of the eight keys, paired from the rows as they came
     unsigned cols[8][C / 2];
@@ -341,8 +373,8 @@ struct PagedTile {
     for (int e = 0; e < 8; e++)
 #pragma unroll
       for (int i = 0; i < C / 2; i++) {
-        if constexpr (QUANT) cols[e][i] = MM<T>::from_fp8(vr[e][i / 2], i % 2);
-        else cols[e][i] = vr[e][i];
+        if constexpr (QUANT) cols[e][i] = MM<T>::from_fp8(x.v[e][i / 2], i % 2);
+        else cols[e][i] = x.v[e][i];
       }
 #pragma unroll
     for (int t = 0; t < C; t++) {
@@ -355,7 +387,7 @@ struct PagedTile {
   }
 };
 
-// One segment's sums over the waves (or pieces) that hold a part of it.  `n` parts: m, l at parts[i * stride + row], [.. + 16 + row],
+// One segment's sums over the waves that hold a part of it.  `n` parts: m, l at parts[i * stride + row], [.. + 16 + row],
 // weighted sums at [.. + 32 + row * ROW + d].  Threads take four columns each.
 template <typename T, int DV, int ROW>
 __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, int b, int h0, int rows, const float* parts, int64_t stride, int n, int threads, bool result,
@@ -388,43 +420,60 @@ __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, int b, int h0
 }
 
 // WHOLE: a workgroup per segment (few keys at most); otherwise equal shares of all units
-template <typename T, bool QUANT, int DQK, int DV, bool WHOLE>
-__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_attn_kernel(PagedAttnArgs a, int least) {
+template <typename T, bool QUANT, int DQK, int DV, int WAVES, int OCC, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES, OCC) void paged_attn_kernel(PagedAttnArgs a, int least) {
   typedef PagedTile<T, QUANT, DQK, DV> Tile;
   constexpr int ROW = DV + 4;  // (heads 4 banks apart)
+  constexpr int UNIT = WAVES * PA_TILE;
   extern __shared__ float lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int segs = a.heads * a.blocks, rep = a.Hq / a.heads;
-  int u, u1, b, at;
+  int u, u1, b, at, per = 0, length;
   if constexpr (WHOLE) {
     b = blockIdx.x / segs;
     at = 0;  // (units are counted from the sequence's first)
+    length = a.lengths[b];
   } else {
-    const Share s = share_of(a, gridDim.x, least, blockIdx.x);
-    u = blockIdx.x * s.per;
-    u1 = min(u + s.per, s.total);
-    if (u >= u1) return;
+    const Share s = share_of<UNIT>(a, gridDim.x, least, blockIdx.x);
+    per = s.per;
+    u = blockIdx.x * per;
+    u1 = min(u + per, s.total);
     b = s.b;
     at = s.at;
+    length = s.length;
   }
-  Keys keys(a, b);
+  Keys keys(a, length);
+  int units = keys.units(UNIT);
   if constexpr (WHOLE) {
-    u = (blockIdx.x - b * segs) * keys.units;
-    u1 = u + keys.units;
+    u = (blockIdx.x - b * segs) * units;
+    u1 = u + units;
+  } else {
+    const int seg = (u - at) / units, begin = at + seg * units, kv = seg / a.blocks, block = seg - kv * a.blocks;
+    if (threadIdx.x == 0) {
+      const bool cut = u < u1 && begin < u && begin >= u - per;
+      const int first = begin / per;
+      reinterpret_cast<SegmentCut*>(a.ws)[blockIdx.x] = {cut ? min(16, rep - 16 * block) : 0, b, kv * rep + 16 * block, first, (begin + units - 1) / per, first * per < begin, {0, 0}};
+    }
   }
   const int stride = 32 + a.rows * ROW;
   float* mine = lds + wave * stride;
   int piece = 2 * blockIdx.x;
   while (u < u1) {
-    const int seg = (u - at) / keys.units, step0 = u - at - seg * keys.units, step1 = min(keys.units, step0 + u1 - u);
+    const int seg = (u - at) / units, step0 = u - at - seg * units, step1 = min(units, step0 + u1 - u);
     const int kv = seg / a.blocks, block = seg - kv * a.blocks, h0 = kv * rep + 16 * block, rows = min(16, rep - 16 * block);
     typename Tile::v8 q[Tile::KS];
     Tile::load_q(a, reinterpret_cast<const T*>(a.q) + b * a.q_b + (h0 + r) * a.q_h, r < rows, q);
     Partial<DV> p;
     p.clear();
-    for (int step = step0; step < step1; step++) {
-      const int key0 = keys.base + (step * PA_WAVES + wave) * PA_TILE;
-      if (key0 < keys.end) Tile::run(a, q, b, kv, key0, keys.first, keys.end, p);
+    const int stop = min(keys.end, keys.base + step1 * UNIT);
+    int key0 = keys.base + (step0 * WAVES + wave) * PA_TILE;
+    typename Tile::Where at_keys = Tile::find(a, b, key0);
+    for (; key0 < stop; key0 += UNIT) {
+      const typename Tile::Where now = at_keys;
+      at_keys = Tile::find(a, b, key0 + UNIT);  // (on its way before the loads of this tile)
+      typename Tile::Data x;
+      Tile::load(a, now, kv, key0, x);
+      Tile::add(a, q, x, keys.first, keys.end, p);
     }
     p.l = groups_sum(p.l);
     if (r < rows) {
@@ -444,80 +493,98 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_attn_kernel(PagedAttnA
         }
     }
     __syncthreads();
-    const bool result = step0 == 0 && step1 == keys.units;
-    join_parts<T, DV, ROW>(a, b, h0, rows, lds, stride, PA_WAVES, 64 * PA_WAVES, result, a.ws + (int64_t)piece * pa_piece_floats(DV));
+    const bool result = step0 == 0 && step1 == units;
+    join_parts<T, DV, ROW>(a, b, h0, rows, lds, stride, WAVES, 64 * WAVES, result, pa_piece(a, gridDim.x, piece, DV));
     piece = 2 * blockIdx.x + 1;
     u += step1 - step0;
     if (u < u1) {
       __syncthreads();
-      if (u - at == keys.units * segs) {
+      if (u - at == units * segs) {
         at = u;
-        keys = Keys(a, ++b);
+        keys = Keys(a, a.lengths[++b]);
+        units = keys.units(UNIT);
       }
     }
   }
 }
 
-// Workgroup w looks at the first unit of share w + 1: where that is inside a segment whose first cut it is, it adds the segment up.
+// Workgroup (w, y) adds up rows of the cut that workgroup w + 1 named: DV / 4 lanes for every SETS-th piece of a row, then the sets
+// through LDS.
 constexpr int PA_JOIN = 256;
-template <typename T, int DV>
-__global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs a, int groups, int least) {
-  const int rep = a.Hq / a.heads, w = blockIdx.x + 1;
-  const Share s = share_of(a, groups, least, w);
-  const int u = w * s.per;
-  if (u >= s.total) return;
-  const Keys keys(a, s.b);
-  const int seg = (u - s.at) / keys.units, begin = s.at + seg * keys.units, end = begin + keys.units;
-  if (begin == u || begin < u - s.per) return;  // no cut, or not its first
-  const int first = begin / s.per, last = (end - 1) / s.per;  // (workgroups)
-  const int kv = seg / a.blocks, block = seg - kv * a.blocks, h0 = kv * rep + 16 * block, rows = min(16, rep - 16 * block);
-  // its pieces: the first workgroup's last one, then the others' first ones
-  const int64_t one = pa_piece_floats(DV);
-  const float* p0 = a.ws + (2 * first + (first * s.per == begin ? 0 : 1)) * one;
-  for (int i = threadIdx.x; i < rows * (DV / 4); i += PA_JOIN) {
-    const int row = i / (DV / 4), d = (i - row * (DV / 4)) * 4;
-    float m = p0[row];
-    for (int k = first + 1; k <= last; k++) m = fmaxf(m, a.ws[2 * k * one + row]);
-    const float base = m == -INFINITY ? 0.f : m;
-    float f = fast_exp2(p0[row] - base), l = f * p0[16 + row];
-    f32x4 o = f * *reinterpret_cast<const f32x4*>(p0 + 32 + row * DV + d);
-    for (int k = first + 1; k <= last; k++) {
-      const float* p = a.ws + 2 * k * one;
-      f = fast_exp2(p[row] - base);
-      l += f * p[16 + row];
-      o += f * *reinterpret_cast<const f32x4*>(p + 32 + row * DV + d);
-    }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(a.out) + s.b * a.o_b + (h0 + row) * a.o_h + d) = pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (d == 0 && a.lse) a.lse[(int64_t)s.b * a.Hq + h0 + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+template <typename T, int DV, int SETS>
+__global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs a, int groups) {
+  constexpr int LANES = DV / 4, ROWS = PA_JOIN / (LANES * SETS);
+  __shared__ float lm[ROWS][SETS], ll[ROWS][SETS];
+  __shared__ f32x4 lo[ROWS][SETS][LANES];
+  const SegmentCut s = reinterpret_cast<const SegmentCut*>(a.ws)[blockIdx.x + 1];
+  const int lane = threadIdx.x % LANES, set = threadIdx.x / LANES % SETS, at = threadIdx.x / (LANES * SETS), row = blockIdx.y * ROWS + at;
+  if (blockIdx.y * ROWS >= (unsigned)s.rows) return;
+  const bool mine = row < s.rows;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+  for (int k = s.first + set; k <= s.last && mine; k += SETS) {
+    const float* p = pa_piece(a, groups, 2 * k + (k == s.first ? s.lead : 0), DV);
+    const float pm = p[row], pl = p[16 + row];
+    const f32x4 po = *reinterpret_cast<const f32x4*>(p + 32 + row * DV + 4 * lane);
+    const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top, f = fast_exp2(m - base), g = fast_exp2(pm - base);
+    l = l * f + pl * g;
+    o = o * f + po * g;
+    m = top;
   }
+  if constexpr (SETS > 1) {
+    if (lane == 0) {
+      lm[at][set] = m;
+      ll[at][set] = l;
+    }
+    lo[at][set][lane] = o;
+    __syncthreads();
+    if (set) return;
+    for (int k = 1; k < SETS; k++) m = fmaxf(m, lm[at][k]);
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < SETS; k++) {
+      const float f = fast_exp2(lm[at][k] - base);
+      l += f * ll[at][k];
+      o += f * lo[at][k][lane];
+    }
+  }
+  if (!mine) return;
+  const int h = s.h0 + row;
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(a.out) + s.b * a.o_b + h * a.o_h + 4 * lane) = pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (lane == 0 && a.lse) a.lse[(int64_t)s.b * a.Hq + h] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
 }
 
 // ---- host --------------------------------------------------------------------------------------
-// Workgroups of a call and the least units each takes.  Where the table has room for no more than `WHOLE_UNITS` units a sequence, a
+// Workgroups of a call and the least units each takes.  Where the table has room for no more than PA_WHOLE keys a sequence, a
 // workgroup takes a whole segment, no piece is left over and no second launch follows.
 struct PagedPlan {
   bool whole;
   int groups, least;
 };
-constexpr int PA_GROUPS = 512, PA_LEAST = 2, PA_WHOLE_UNITS = 2;
+constexpr int PA_WAVES = 4, PA_GROUPS = 512, PA_GROUPS_8BIT = 768, PA_LEAST = 1, PA_WHOLE = 512;
 inline PagedPlan paged_plan(const tp_kv_cache* c, int B, int Hq) {
-  const int64_t segs = (int64_t)B * c->heads * ((Hq / c->heads + 15) / 16);
-  const int64_t units = ((int64_t)c->table_width * c->page_size + PA_TILE + PA_UNIT - 1) / PA_UNIT;
-  if (units <= PA_WHOLE_UNITS) return {true, (int)segs, 1};
-  return {false, (int)std::min<int64_t>(PA_GROUPS, (segs * units + PA_LEAST - 1) / PA_LEAST), PA_LEAST};
+  const int64_t segs = (int64_t)B * c->heads * ((Hq / c->heads + 15) / 16), keys = (int64_t)c->table_width * c->page_size;
+  if (keys <= PA_WHOLE) return {true, (int)segs, 1};
+  const int64_t units = (keys + PA_TILE) / (PA_WAVES * PA_TILE) + 1, most = c->dtype == TP_FP8 ? PA_GROUPS_8BIT : PA_GROUPS;
+  return {false, (int)std::min(most, (segs * units + PA_LEAST - 1) / PA_LEAST), PA_LEAST};
 }
 
 template <typename T, bool QUANT, int DQK, int DV>
 int paged_launch(const PagedAttnArgs& a, const PagedPlan& plan, hipStream_t st) {
   const int lds = PA_WAVES * (32 + a.rows * (DV + 4)) * 4;
-  const auto kern = plan.whole ? paged_attn_kernel<T, QUANT, DQK, DV, true> : paged_attn_kernel<T, QUANT, DQK, DV, false>;
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    TP_REQUIRE(e == hipSuccess, TP_ERR_LAUNCH, "tp_paged_attn: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
-  }
+  const auto kern = plan.whole ? paged_attn_kernel<T, QUANT, DQK, DV, PA_WAVES, QUANT ? 3 : 2, true> : paged_attn_kernel<T, QUANT, DQK, DV, PA_WAVES, QUANT ? 3 : 2, false>;
   kern<<<plan.groups, 64 * PA_WAVES, lds, st>>>(a, plan.least);
-  if (!plan.whole && plan.groups > 1) paged_attn_join_kernel<T, DV><<<plan.groups - 1, PA_JOIN, 0, st>>>(a, plan.groups, plan.least);
+  if (!plan.whole && plan.groups > 1) {
+    const int per_row = PA_JOIN / (DV / 4);
+    // many workgroups to a segment: eight threads share out the pieces of four columns
+    if (plan.groups > 4 * a.B * a.heads * a.blocks)
+      paged_attn_join_kernel<T, DV, 8><<<dim3(plan.groups - 1, (a.rows * 8 + per_row - 1) / per_row), PA_JOIN, 0, st>>>(a, plan.groups);
+    else
+      paged_attn_join_kernel<T, DV, 1><<<dim3(plan.groups - 1, (a.rows + per_row - 1) / per_row), PA_JOIN, 0, st>>>(a, plan.groups);
+  }
   return check_launch("tp_paged_attn");
 }
 
@@ -525,9 +592,9 @@ int paged_launch(const PagedAttnArgs& a, const PagedPlan& plan, hipStream_t st) 
 
 extern "C" size_t tp_paged_attn_workspace_bytes(const tp_kv_cache* c, int B, int Hq, int dtype) {
   using namespace tp;
-  if (check_cache(c, dtype, B, "tp_paged_attn_workspace_bytes") || Hq < 1 || Hq % c->heads || dtype == TP_F32) return 0;
+  if (check_cache(c, dtype, B, "tp_paged_attn_workspace_bytes") != TP_OK || Hq < 1 || Hq % c->heads || dtype == TP_F32) return 0;
   const PagedPlan plan = paged_plan(c, B, Hq);
-  return plan.whole ? 0 : sizeof(float) * 2 * plan.groups * pa_piece_floats(c->v_dim);
+  return plan.whole ? 0 : plan.groups * (sizeof(SegmentCut) + sizeof(float) * 2 * pa_piece_floats(c->v_dim));
 }
 
 extern "C" int tp_paged_attn(const tp_kv_cache* c, const void* q, const int32_t* lengths, void* out, float* lse, void* ws, int B, int Hq,
@@ -545,7 +612,7 @@ extern "C" int tp_paged_attn(const tp_kv_cache* c, const void* q, const int32_t*
   for (int i = 0; i < 2; i++)
     TP_REQUIRE(q_strides[i] * e % 16 == 0 && o_strides[i] * e % 16 == 0, TP_ERR_BAD_ARG, "tp_paged_attn: strides must keep rows 16-byte aligned");
   TP_REQUIRE((int64_t)B * Hq < (1ll << 24), TP_ERR_UNSUPPORTED, "tp_paged_attn: too many rows");
-  TP_REQUIRE((int64_t)B * c->heads * ((Hq / c->heads + 15) / 16) * (((int64_t)c->table_width * c->page_size) / PA_UNIT + 2) < (1ll << 31) - PA_GROUPS,
+  TP_REQUIRE((int64_t)B * c->heads * ((Hq / c->heads + 15) / 16) * (((int64_t)c->table_width * c->page_size) / (PA_WAVES * PA_TILE) + 2) < (1ll << 30),
              TP_ERR_UNSUPPORTED, "tp_paged_attn: the table covers too many keys");
   const int rep = Hq / c->heads;
   const PagedAttnArgs a{rows_of(c, false), rows_of(c, true), table_of(c), q, lengths, out, lse, (float*)ws, q_strides[0], q_strides[1], o_strides[0],
