@@ -477,7 +477,7 @@ int tp_paged_attn(const tp_kv_cache* cache, const void* q, const int32_t* length
  *   logprob: log(w / sum of all kept)
  * A temperature that is not positive takes the first of the largest logits.  A row without a logit above -inf gives token -1 and
  * logprob -inf.  Each of temperatures, top_ks, top_ps, min_ps is (B) or NULL: then the value beside it holds for all rows.
- * ws: tp_sample_workspace_bytes bytes (may be 0), 16-byte aligned. */
+ * ws: tp_sample_workspace_bytes bytes, 16-byte aligned. */
 size_t tp_sample_workspace_bytes(int B, int V);
 int tp_sample(const void* logits, const float* uniform, const float* temperatures, const int32_t* top_ks,
               const float* top_ps, const float* min_ps, float temperature, int top_k, float top_p, float min_p,

@@ -559,24 +559,33 @@ __global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs 
 
 // ---- host --------------------------------------------------------------------------------------
 // Workgroups of a call and the least units each takes.  Where the table has room for no more than PA_WHOLE keys a sequence, a
-// workgroup takes a whole segment, no piece is left over and no second launch follows.
+// workgroup (of more waves) takes a whole segment, no piece is left over and no second launch follows.
+//   us, one CU's waves 4 : 8, up to 512 keys: one sequence of 461 keys and 8 kv heads 8.95 : 8.83, 16 of 20 to 300 9.8 : 9.0,
+//   64 of 20 to 300 13.1 : 15.2: eight waves where the segments do not fill the CUs, four where they do.
 struct PagedPlan {
   bool whole;
-  int groups, least;
+  int waves, groups, least;
 };
-constexpr int PA_WAVES = 4, PA_GROUPS = 512, PA_GROUPS_8BIT = 768, PA_LEAST = 1, PA_WHOLE = 512;
+constexpr int PA_WAVES = 4, PA_WHOLE_FEW = 8, PA_CUS = 256, PA_GROUPS = 512, PA_GROUPS_8BIT = 768, PA_LEAST = 1, PA_WHOLE = 512;
 inline PagedPlan paged_plan(const tp_kv_cache* c, int B, int Hq) {
   const int64_t segs = (int64_t)B * c->heads * ((Hq / c->heads + 15) / 16), keys = (int64_t)c->table_width * c->page_size;
-  if (keys <= PA_WHOLE) return {true, (int)segs, 1};
+  if (keys <= PA_WHOLE) return {true, segs <= PA_CUS ? PA_WHOLE_FEW : PA_WAVES, (int)segs, 1};
   const int64_t units = (keys + PA_TILE) / (PA_WAVES * PA_TILE) + 1, most = c->dtype == TP_FP8 ? PA_GROUPS_8BIT : PA_GROUPS;
-  return {false, (int)std::min(most, (segs * units + PA_LEAST - 1) / PA_LEAST), PA_LEAST};
+  return {false, PA_WAVES, (int)std::min(most, (segs * units + PA_LEAST - 1) / PA_LEAST), PA_LEAST};
 }
 
 template <typename T, bool QUANT, int DQK, int DV>
 int paged_launch(const PagedAttnArgs& a, const PagedPlan& plan, hipStream_t st) {
-  const int lds = PA_WAVES * (32 + a.rows * (DV + 4)) * 4;
-  const auto kern = plan.whole ? paged_attn_kernel<T, QUANT, DQK, DV, PA_WAVES, QUANT ? 3 : 2, true> : paged_attn_kernel<T, QUANT, DQK, DV, PA_WAVES, QUANT ? 3 : 2, false>;
-  kern<<<plan.groups, 64 * PA_WAVES, lds, st>>>(a, plan.least);
+  constexpr int OCC = QUANT ? 3 : 2;  // (waves per SIMD)
+  const int lds = plan.waves * (32 + a.rows * (DV + 4)) * 4;
+  const auto kern = !plan.whole                  ? paged_attn_kernel<T, QUANT, DQK, DV, PA_WAVES, OCC, false>
+                    : plan.waves == PA_WHOLE_FEW ? paged_attn_kernel<T, QUANT, DQK, DV, PA_WHOLE_FEW, 2, true>
+                                                 : paged_attn_kernel<T, QUANT, DQK, DV, PA_WAVES, OCC, true>;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    TP_REQUIRE(e == hipSuccess, TP_ERR_LAUNCH, "tp_paged_attn: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
+  }
+  kern<<<plan.groups, 64 * plan.waves, lds, st>>>(a, plan.least);
   if (!plan.whole && plan.groups > 1) {
     const int per_row = PA_JOIN / (DV / 4);
     // many workgroups to a segment: eight threads share out the pieces of four columns

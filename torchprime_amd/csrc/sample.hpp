@@ -3,13 +3,22 @@
 //   w = 2^((l - m) c), m the largest logit, c = log2(e) / temperature; 1 where l == m;   then (w + 2^-12) - 2^-12 in fp32
 //
 // The last step makes every weight a multiple of 2^-35 (w is at most 1), so sums of up to 2^18 of them are exact in fp64: they
-// come out the same in any order and over any split of the row, and so do the token and every cut through the distribution.
-// Weights below 2^-36 become zero; such tokens are never drawn.
+// come out the same in any order and over any split of the row, and so do the token and every cut through the distribution;
+// atomics may add them up.  Weights below 2^-36 become zero; such tokens are never drawn.
 //
-// Tokens are ranked by falling logit, the lower index first among equals.  Every filter keeps a beginning of that order, which a
-// logit and a number of its equals describe (Cut); the cut of top-k (by count) and of top-p (by weight) is found digit by
-// digit over the 32 bits of an order-preserving integer key of the logit.  The draw walks the kept tokens by index, which needs no
-// sort: a sum per stretch of the row, then the stretch that the drawn weight falls into.
+// Tokens are ranked by falling logit, the lower index first among equals.  Every filter but min-p keeps a beginning of that order,
+// which its last token (logit, index) describes; min-p is a bound on the weight itself.  The draw walks the kept tokens by index,
+// which needs no sort of the row: a sum per cell of the row (16 vectors of 16 bytes), then the cell that the drawn weight falls into.
+//
+// Three launches, the second only where a row may need it:
+//   sample_cells_kernel  the row split over workgroups: the largest logit of each cell.  It reads everything, once, and is bound by HBM.
+//   sample_mass_kernel   rows without top-k: the weight of each cell (no filter at all), or of each of 2048 stretches of the logit's
+//                        range (top-p): the row again, from the caches unless the batch is larger than they are.
+//   sample_pick_kernel   a workgroup per row.  A short list of tokens decides: with top-k, those not below the k-th largest of the
+//                        cells' largest logits (at least k tokens are not), found in the few cells that hold any; with top-p, those of the
+//                        one stretch that the cut lies in, in one more walk over the row; with min-p, those that have the weight.  The list
+//                        is sorted by rank, cut, and drawn from.  Where it would not fit (thousands of equals, top-k in the
+//                        thousands), the cut is found digit by digit over an order-preserving integer key of the logits, slower.
 #pragma once
 #include <float.h>
 
@@ -20,6 +29,12 @@ namespace tp {
 constexpr float SAMPLE_LOG2E = 1.4426950408889634f;
 constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / WAVE;
 constexpr int SAMPLE_MOST = 1 << 18;  // logits per row
+constexpr int SAMPLE_CELL = 16;       // vectors of 16 bytes, one per lane of a group of 16
+constexpr int SAMPLE_CELLS = SAMPLE_MOST / 4 / SAMPLE_CELL + 2;
+constexpr int SAMPLE_LIST = 1024;     // tokens that are sorted at most
+constexpr int SAMPLE_TOP_K = 640;     // the list takes top-k up to half the cells, and this: about C log(1 / (1 - k / C)) of C cells' tokens
+constexpr int SAMPLE_BINS = 2048;     // over weights from 1 down to 2^-36
+constexpr float SAMPLE_BIN = SAMPLE_BINS / 36.5f;
 
 struct SampleArgs {
   const void* logits;
@@ -29,9 +44,17 @@ struct SampleArgs {
   int top_k;
   int64_t* tokens;
   float* logprobs;
+  char* ws;
   int64_t row_stride;
   int V;
+  // of row r: the bins, the cells' weights, the cells' largest logits
+  static constexpr int64_t ws_row(int cells) { return (SAMPLE_BINS * 8 + (int64_t)cells * 12 + 15) / 16 * 16; }
+  int cells;
+  __device__ __forceinline__ double* bins(int r) const { return reinterpret_cast<double*>(ws + r * ws_row(cells)); }
+  __device__ __forceinline__ double* masses(int r) const { return bins(r) + SAMPLE_BINS; }
+  __device__ __forceinline__ float* maxima(int r) const { return reinterpret_cast<float*>(masses(r) + cells); }
 };
+inline int sample_cells(int V) { return (V / 4 + 2 + SAMPLE_CELL - 1) / SAMPLE_CELL; }  // at most, for any type and address
 
 // larger logit, larger key; -0 and +0 have the same
 __device__ __forceinline__ unsigned sample_key(float l) {
@@ -45,28 +68,49 @@ __device__ __forceinline__ float sample_logit(unsigned key) {
 // what a row's weights depend on
 struct Weights {
   float m, c;
-  __device__ __forceinline__ float operator()(float l) const {
-    const float w = l == m ? 1.f : __builtin_amdgcn_exp2f((l - m) * c);
-    return (w + 0x1p-12f) - 0x1p-12f;
+  __device__ __forceinline__ Weights(float largest, float temperature) : m(largest), c(fmaxf(SAMPLE_LOG2E / temperature, FLT_MIN)) {}  // (c = 0 would not keep -inf out)
+  __device__ __forceinline__ float power(float l) const { return l == m ? 0.f : (l - m) * c; }
+  __device__ __forceinline__ float of_power(float x) const { return (__builtin_amdgcn_exp2f(x) + 0x1p-12f) - 0x1p-12f; }
+  __device__ __forceinline__ float operator()(float l) const { return of_power(power(l)); }
+  // falls as the logit rises; beyond the last bin nothing has a weight
+  __device__ __forceinline__ static int bin(float x) { return (int)fminf(-x * SAMPLE_BIN, (float)SAMPLE_BINS); }
+};
+
+enum SampleKind { GREEDY, LIST, TOP_K, TOP_P, MIN_P, ALL, DIGITS };
+struct Settings {
+  float temperature, top_p, min_p;
+  int top_k;  // 0: all
+  SampleKind kind;
+  __device__ __forceinline__ Settings(const SampleArgs& a, int row, int cells) {
+    temperature = a.temperatures ? a.temperatures[row] : a.temperature;
+    top_k = a.top_ks ? a.top_ks[row] : a.top_k;
+    top_p = fminf(fmaxf(a.top_ps ? a.top_ps[row] : a.top_p, 0.f), 1.f);
+    min_p = fminf(fmaxf(a.min_ps ? a.min_ps[row] : a.min_p, 0.f), 1.f);
+    if (top_k <= 0 || top_k >= a.V) top_k = 0;
+    if (!(temperature > 0.f) || top_k == 1 || top_p <= 0.f) kind = GREEDY;
+    else if (a.V <= SAMPLE_LIST) kind = LIST;
+    else if (top_k) kind = top_k <= min(cells / 2, SAMPLE_TOP_K) ? TOP_K : DIGITS;
+    else if (top_p < 1.f) kind = TOP_P;
+    else kind = min_p > 0.f ? MIN_P : ALL;
   }
 };
 
-// A beginning of the ranking: every key above `key`, and the first `ties` tokens (by index) that have it.
-struct Cut {
-  unsigned key;
-  int ties;
-};
-
-// The logits of a row, 16 bytes at a time from 16-byte addresses; elements outside the row are -inf.
+// The logits of a row, 16 bytes at a time from 16-byte addresses; elements outside the row, and NaN, are -inf.
 template <typename T>
 struct Row {
   static constexpr int E = 16 / sizeof(T);
   const T* base;  // 16-byte aligned, `lead` elements before the row's first
   int lead, V;
-  __device__ __forceinline__ Row(const T* p, int v) : lead((int)(((size_t)p & 15) / sizeof(T))), V(v) { base = p - lead; }
+  __device__ __forceinline__ Row(const SampleArgs& a, int row) : V(a.V) {
+    const T* p = reinterpret_cast<const T*>(a.logits) + row * a.row_stride;
+    lead = (int)(((size_t)p & 15) / sizeof(T));
+    base = p - lead;
+  }
   __device__ __forceinline__ int vectors() const { return (V + lead + E - 1) / E; }
+  __device__ __forceinline__ int cells() const { return (vectors() + SAMPLE_CELL - 1) / SAMPLE_CELL; }
+  __device__ __forceinline__ int index(int vec, int e) const { return vec * E + e - lead; }
   __device__ __forceinline__ void load(int vec, float (&x)[E]) const {
-    const int i0 = vec * E - lead;
+    const int i0 = index(vec, 0);
     if (i0 >= 0 && i0 + E <= V) {
       load_f<T, E>(base + (int64_t)vec * E, x);
     } else {
@@ -83,70 +127,352 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
+__device__ __forceinline__ double cell_sum(double v) {
+#pragma unroll
+  for (int o = SAMPLE_CELL / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
 
-template <typename T>
-__global__ __launch_bounds__(SAMPLE_THREADS) void sample_rows_kernel(SampleArgs a) {
+// ------------------------------------------------------------------------------------------------
+constexpr int SAMPLE_SPLIT = 256;  // threads of a workgroup that takes a part of a row
+template <typename T, int U>
+__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
-  __shared__ double mass[256];
-  __shared__ int count[256];
-  __shared__ double stretch[SAMPLE_MOST / WAVE / E + 2];
-  __shared__ float wm[SAMPLE_WAVES];
-  __shared__ int wi[SAMPLE_WAVES];
-  __shared__ double wd[SAMPLE_WAVES];
-  __shared__ unsigned found_key;
-  __shared__ int found_at;
-  __shared__ double found_before;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Row<T> x(reinterpret_cast<const T*>(a.logits) + row * a.row_stride, a.V);
-  const int nv = x.vectors(), stretches = (nv + WAVE - 1) / WAVE;
-
-  // the largest logit, its first index
-  float m = -INFINITY;
-  int at = 0x7fffffff;
-  for (int v = tid; v < nv; v += SAMPLE_THREADS) {
-    float l[E];
-    x.load(v, l);
+  const int row = blockIdx.y;
+  const Row<T> x(a, row);
+  const int nv = x.vectors(), v0 = blockIdx.x * (SAMPLE_SPLIT * U) + threadIdx.x;
+  float l[U][E];
 #pragma unroll
-    for (int e = 0; e < E; e++)
-      if (l[e] > m) {
-        m = l[e];
-        at = v * E + e - x.lead;
-      }
+  for (int u = 0; u < U; u++)
+    if (v0 + u * SAMPLE_SPLIT < nv) x.load(v0 + u * SAMPLE_SPLIT, l[u]);
+  float* out = a.maxima(row);
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const int v = v0 + u * SAMPLE_SPLIT;
+    float m = -INFINITY;
+    if (v < nv) {
+#pragma unroll
+      for (int e = 0; e < E; e++) m = fmaxf(m, l[u][e]);
+    }
+#pragma unroll
+    for (int o = SAMPLE_CELL / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (threadIdx.x % SAMPLE_CELL == 0 && v < nv) out[v / SAMPLE_CELL] = m;
   }
+  // cleared for the next kernel to add to
+  for (int i = blockIdx.x * SAMPLE_SPLIT + threadIdx.x; i < SAMPLE_BINS; i += gridDim.x * SAMPLE_SPLIT) a.bins(row)[i] = 0.;
+}
+
+template <typename T, int U>
+__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a) {
+  constexpr int E = Row<T>::E;
+  __shared__ double bins[SAMPLE_BINS];
+  __shared__ float wm[SAMPLE_SPLIT / WAVE];
+  const int row = blockIdx.y, tid = threadIdx.x;
+  const Row<T> x(a, row);
+  const int nv = x.vectors(), cells = x.cells(), v0 = blockIdx.x * (SAMPLE_SPLIT * U) + tid;
+  const Settings s(a, row, cells);
+  if (s.kind != TOP_P && s.kind != ALL) return;
+  float m = -INFINITY;
+  const float* maxima = a.maxima(row);
+  for (int i = tid; i < cells; i += SAMPLE_SPLIT) m = fmaxf(m, maxima[i]);
+  m = wave_max(m);
+  if (tid % WAVE == 0) wm[tid / WAVE] = m;
+  for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT) bins[i] = 0.;
+  __syncthreads();
+  for (int i = 0; i < SAMPLE_SPLIT / WAVE; i++) m = fmaxf(m, wm[i]);
+  const Weights weight(m, s.temperature);
+  for (int u = 0; u < U; u++) {
+    const int v = v0 + u * SAMPLE_SPLIT;
+    double sum = 0.;
+    if (v < nv) {
+      float l[E];
+      x.load(v, l);
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor(m, o, 64);
-    const int at2 = __shfl_xor(at, o, 64);
-    if (m2 > m || (m2 == m && at2 < at)) {
-      m = m2;
-      at = at2;
+      for (int e = 0; e < E; e++) {
+        const float p = weight.power(l[e]), w = weight.of_power(p);
+        if (s.kind == ALL) sum += (double)w;
+        else if (w > 0.f) atomicAdd(&bins[Weights::bin(p)], (double)w);
+      }
+    }
+    if (s.kind == ALL) {
+      sum = cell_sum(sum);
+      if (tid % SAMPLE_CELL == 0 && v < nv) a.masses(row)[v / SAMPLE_CELL] = sum;
     }
   }
-  if (lane == 0) {
-    wm[wave] = m;
-    wi[wave] = at;
+  if (s.kind == ALL) return;
+  __syncthreads();
+  double* out = a.bins(row);
+  for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT)
+    if (bins[i] > 0.) __hip_atomic_fetch_add(&out[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // (exact, so in any order)
+}
+
+// ------------------------------------------------------------------------------------------------
+struct PickLds {
+  double mass[SAMPLE_CELLS];
+  float maxima[SAMPLE_CELLS];
+  uint64_t list[SAMPLE_LIST];
+  double wd[SAMPLE_WAVES];
+  float wf[SAMPLE_WAVES];
+  int count, at;
+  double begin;
+  uint64_t last;
+};
+
+// the sum of v over the threads before this one and itself; `all` over all.  For the whole workgroup.
+__device__ __forceinline__ double group_scan(double v, PickLds& s, double& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(v, o, 64);
+    if (lane >= o) v += y;
+  }
+  if (lane == 63) s.wd[wave] = v;
+  __syncthreads();
+  double before = 0.;
+  all = 0.;
+#pragma unroll
+  for (int i = 0; i < SAMPLE_WAVES; i++) {
+    before += i < wave ? s.wd[i] : 0.;
+    all += s.wd[i];
   }
   __syncthreads();
-  for (int i = 0; i < SAMPLE_WAVES; i++)
-    if (wm[i] > m || (wm[i] == m && wi[i] < at)) {
-      m = wm[i];
-      at = wi[i];
-    }
-  const float temperature = a.temperatures ? a.temperatures[row] : a.temperature;
-  if (m == -INFINITY || !(temperature > 0.f)) {  // (the same for the whole workgroup)
-    if (tid == 0) {
-      a.tokens[row] = m == -INFINITY ? -1 : at;
-      a.logprobs[row] = m == -INFINITY ? -INFINITY : 0.f;
-    }
-    return;
-  }
-  const Weights weight{m, fmaxf(SAMPLE_LOG2E / temperature, FLT_MIN)};  // (not 0: an infinite temperature keeps -inf out)
+  return before + v;
+}
 
+// list[0, n) in rising order; places from n to the next power of two are filled up
+__device__ __forceinline__ void sort_list(PickLds& s, int n) {
+  int size = 64;
+  while (size < n) size *= 2;
+  for (int i = n + threadIdx.x; i < size; i += SAMPLE_THREADS) s.list[i] = ~0ull;
+  __syncthreads();
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += SAMPLE_THREADS) {
+        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const uint64_t x = s.list[lo], y = s.list[hi];
+        if ((x > y) == ((lo & k) == 0)) {
+          s.list[lo] = y;
+          s.list[hi] = x;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+template <typename T>
+struct Picker {
+  static constexpr int E = Row<T>::E;
+  const SampleArgs& a;
+  PickLds& s;
+  const int row, tid, lane, wave;
+  const Row<T> x;
+  const int nv, cells;
+  const Settings set;
+  float m;
+
+  __device__ __forceinline__ Picker(const SampleArgs& args, PickLds& lds)
+      : a(args), s(lds), row(blockIdx.x), tid(threadIdx.x), lane(tid & 63), wave(tid >> 6), x(args, blockIdx.x), nv(x.vectors()), cells(x.cells()),
+        set(args, blockIdx.x, cells) {
+    m = -INFINITY;
+    const float* maxima = a.maxima(row);
+    for (int i = tid; i < cells; i += SAMPLE_THREADS) {
+      const float c = maxima[i];
+      s.maxima[i] = c;
+      m = fmaxf(m, c);
+    }
+    m = wave_max(m);
+    if (lane == 0) s.wf[wave] = m;
+    if (tid == 0) {
+      s.count = 0;
+      s.at = 0x7fffffff;
+    }
+    __syncthreads();
+    for (int i = 0; i < SAMPLE_WAVES; i++) m = fmaxf(m, s.wf[i]);
+  }
+
+  __device__ __forceinline__ void answer(int token, double chosen, double all) const {
+    a.tokens[row] = token;
+    a.logprobs[row] = (float)log(chosen / all);
+  }
+
+  // f(vector, its logits) of the cells that `wants`; every lane of a cell's 16 together
+  template <typename W, typename F>
+  __device__ __forceinline__ void visit(W&& wants, F&& f) const {
+    for (int c = tid / SAMPLE_CELL; c < cells; c += SAMPLE_THREADS / SAMPLE_CELL) {
+      if (!wants(c)) continue;
+      const int v = c * SAMPLE_CELL + tid % SAMPLE_CELL;
+      float l[E];
+      if (v < nv) x.load(v, l);
+      else
+#pragma unroll
+        for (int e = 0; e < E; e++) l[e] = -INFINITY;
+      f(c, v, l);
+    }
+  }
+
+  // the first index of the largest logit
+  __device__ __forceinline__ void greedy() const {
+    visit([&](int c) { return s.maxima[c] == m; },
+          [&](int, int v, const float (&l)[E]) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+              if (l[e] == m) atomicMin(&s.at, x.index(v, e));
+          });
+    __syncthreads();
+    if (tid == 0) answer(s.at, 1., 1.);
+  }
+
+  // Tokens for the list, ranked: the inverted key above the index
+  __device__ __forceinline__ void push(float l, int i) const {
+    const int at = atomicAdd(&s.count, 1);
+    if (at < SAMPLE_LIST) s.list[at] = (uint64_t)~sample_key(l) << 32 | (unsigned)i;
+  }
+  __device__ __forceinline__ float listed(int at) const { return sample_logit(~(unsigned)(s.list[at] >> 32)); }
+
+  // a logit that at least k tokens reach: not above the k-th largest of the cells' maxima, in steps of 1/1024 of their range
+  __device__ __forceinline__ float pivot(int k) const {
+    int* hist = reinterpret_cast<int*>(s.mass);
+    float lo = INFINITY;
+    for (int i = tid; i < cells; i += SAMPLE_THREADS)
+      if (s.maxima[i] > -INFINITY) lo = fminf(lo, s.maxima[i]);
+    lo = -wave_max(-lo);
+    for (int i = tid; i < 1024; i += SAMPLE_THREADS) hist[i] = 0;
+    __syncthreads();  // (the maxima's reduction has been read)
+    if (lane == 0) s.wf[wave] = lo;
+    __syncthreads();
+    for (int i = 0; i < SAMPLE_WAVES; i++) lo = fminf(lo, s.wf[i]);
+    const float step = (m - lo) * (1.f / 1023.f);
+    const auto bin = [&](float l) { return step > 0.f && step < INFINITY ? 1023 - min(1023, (int)((l - lo) / step)) : 0; };
+    for (int i = tid; i < cells; i += SAMPLE_THREADS)
+      if (s.maxima[i] > -INFINITY) atomicAdd(&hist[bin(s.maxima[i])], 1);
+    __syncthreads();
+    // (cells with anything in them may be fewer than k: then the pivot is the smallest, and the list may come out too long)
+    double all;
+    const double n = tid < 1024 ? (double)hist[tid] : 0., upto = group_scan(n, s, all);
+    if (upto >= k && upto - n < k) s.at = tid;
+    __syncthreads();
+    const int b = s.at;
+    float p = m;
+    if (all < k) p = -INFINITY;
+    else
+      for (int i = tid; i < cells; i += SAMPLE_THREADS)
+        if (s.maxima[i] > -INFINITY && bin(s.maxima[i]) <= b) p = fminf(p, s.maxima[i]);
+    p = -wave_max(-p);
+    if (lane == 0) s.wf[wave] = p;
+    __syncthreads();
+    for (int i = 0; i < SAMPLE_WAVES; i++) p = fminf(p, s.wf[i]);
+    return p;
+  }
+
+  // Of the sorted list, behind tokens of weight `before`: the last token kept by top-k and top-p (goal < 0: of the list's own weight)
+  __device__ __forceinline__ uint64_t cut(const Weights& weight, int n, int k, double before, double goal) const {
+    const int most = k ? min(k, n) : n;
+    const double w = tid < most ? (double)weight(listed(tid)) : 0.;
+    double all;
+    const double upto = before + group_scan(w, s, all);
+    if (goal < 0.) goal = set.top_p < 1.f ? (double)set.top_p * all : INFINITY;
+    // kept: what has less than the goal before it (weights that are zero stay out of the draw by themselves)
+    const bool kept = tid < most && (tid == 0 || upto - w < goal);
+    const bool next = tid + 1 < most && upto < goal;
+    if (kept && !next) s.last = s.list[tid];
+    __syncthreads();
+    return s.last;
+  }
+
+  // Draws from the list (`n` sorted by rank, those up to `last` kept)
+  __device__ __forceinline__ void draw_listed(const Weights& weight, int n, uint64_t last) const {
+    // by index: the kept ones only
+    uint64_t mine = ~0ull;
+    if (tid < n && s.list[tid] <= last && weight(listed(tid)) >= set.min_p) mine = (s.list[tid] << 32) | (s.list[tid] >> 32);
+    const int kept = __syncthreads_count(mine != ~0ull);
+    // (with min-p or without, they are a beginning of the list, but for weights that the hardware's exponential does not order)
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    if (mine != ~0ull) s.list[atomicAdd(&s.count, 1)] = mine;
+    __syncthreads();
+    sort_list(s, kept);
+    const double w = tid < kept ? (double)weight(sample_logit(~(unsigned)s.list[tid])) : 0.;
+    double all;
+    const double upto = group_scan(w, s, all);
+    const double goal = (double)fminf(fmaxf(a.uniform[row], 0.f), 0x1.fffffep-1f) * all;
+    if (w > 0. && upto > goal && upto - w <= goal) answer((int)(s.list[tid] >> 32), w, all);
+  }
+
+  // Draws from the whole row: cells' weights in s.mass, kept(l, i) a token's weight
+  template <typename K>
+  __device__ __forceinline__ void draw_cells(K&& kept) const {
+    constexpr int PER = (SAMPLE_CELLS + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
+    double w[PER], sum = 0., all;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      w[i] = tid * PER + i < cells ? s.mass[tid * PER + i] : 0.;
+      sum += w[i];
+    }
+    const double upto = group_scan(sum, s, all);
+    const double goal = (double)fminf(fmaxf(a.uniform[row], 0.f), 0x1.fffffep-1f) * all;
+    if (upto > goal && upto - sum <= goal) {  // (one thread: sums are exact)
+      double begin = upto - sum;
+      int c = tid * PER;
+#pragma unroll
+      for (int i = 0; i < PER - 1; i++)
+        if (c == tid * PER + i && begin + w[i] <= goal) {
+          begin += w[i];
+          c++;
+        }
+      s.at = c;
+      s.begin = begin;
+    }
+    __syncthreads();
+    if (tid >= SAMPLE_CELL) return;
+    const int v = s.at * SAMPLE_CELL + tid;
+    const double begin = s.begin;
+    float l[E];
+    double token[E];
+    sum = 0.;
+    if (v < nv) x.load(v, l);
+#pragma unroll
+    for (int e = 0; e < E; e++) sum += token[e] = v < nv ? kept(l[e], x.index(v, e)) : 0.;
+    double here = sum;
+#pragma unroll
+    for (int o = 1; o < SAMPLE_CELL; o <<= 1) {
+      const double y = __shfl_up(here, o, SAMPLE_CELL);
+      if (tid >= o) here += y;
+    }
+    double left = begin + (here - sum);
+    if (!(left + sum > goal && left <= goal)) return;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if (left <= goal && left + token[e] > goal) answer(x.index(v, e), token[e], all);
+      left += token[e];
+    }
+  }
+
+  // The weight of kept(l, i) in every cell
+  template <typename K>
+  __device__ __forceinline__ void weigh_cells(K&& kept) const {
+    visit([](int) { return true; },
+          [&](int c, int v, const float (&l)[E]) {
+            double sum = 0.;
+#pragma unroll
+            for (int e = 0; e < E; e++) sum += kept(l[e], x.index(v, e));
+            sum = cell_sum(sum);
+            if (tid % SAMPLE_CELL == 0) s.mass[c] = sum;
+          });
+    __syncthreads();
+  }
+
+  // ---- the cut by digits, over the whole row ----
+  struct Digits {
+    unsigned key;
+    int ties;  // tokens of that key, the first by index
+  };
   // the cut that keeps the first `goal_n` tokens, or the first tokens with a weight of goal_w
-  const auto find = [&](bool by_count, int goal_n, double goal_w) {
+  __device__ __forceinline__ Digits find(const Weights& weight, bool by_count, int goal_n, double goal_w) const {
+    double* mass = s.mass;
+    int* count = reinterpret_cast<int*>(s.mass + 256);
     unsigned prefix = 0;
-    double w_before = 0.;
-    int n_before = 0;
+    double before = 0.;
+    const double goal = by_count ? (double)goal_n : goal_w;
     for (int shift = 24; shift >= 0; shift -= 8) {
       for (int i = tid; i < 256; i += SAMPLE_THREADS) {
         mass[i] = 0.;
@@ -162,7 +488,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_rows_kernel(SampleArgs 
           if (shift < 24 && (key >> (shift + 8)) != (prefix >> (shift + 8))) continue;
           const unsigned digit = key >> shift & 255u;
           if (by_count) atomicAdd(&count[digit], 1);
-          else atomicAdd(&mass[digit], (double)weight(l[e]));
+          else if (const float w = weight(l[e]); w > 0.f) atomicAdd(&mass[digit], (double)w);
         }
       }
       __syncthreads();
@@ -175,174 +501,206 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_rows_kernel(SampleArgs 
           const double y = __shfl_up(upto, o, 64);
           if (lane >= o) upto += y;
         }
-        const double goal = by_count ? (double)goal_n : goal_w, before = by_count ? (double)n_before : w_before;
         double begin = before + (upto - sum);
         const uint64_t reached = __ballot(before + upto >= goal);
         const int first = reached ? __ffsll((unsigned long long)reached) - 1 : 63;
         if (lane == first) {
           int i = 0;
           for (; i < 3 && begin + w[i] < goal; i++) begin += w[i];
-          found_key = prefix | (unsigned)(255 - 4 * lane - i) << shift;
-          found_before = begin;
+          s.at = (int)(prefix | (unsigned)(255 - 4 * lane - i) << shift);
+          s.begin = begin;
         }
       }
       __syncthreads();
-      prefix = found_key;
-      if (by_count) n_before = (int)found_before;
-      else w_before = found_before;
+      prefix = (unsigned)s.at;
+      before = s.begin;
       __syncthreads();
     }
-    Cut cut{prefix, 0};
-    if (by_count) {
-      cut.ties = prefix == sample_key(-INFINITY) ? 0 : goal_n - n_before;  // (what is -inf has no weight)
-    } else {
-      // equals have one weight: the j-th (from 0) is kept where what stands before it is below the goal
-      const double w = (double)weight(sample_logit(prefix));
-      double n = w > 0. ? ceil((goal_w - w_before) / w) : 1.;
-      while (n > 1. && !(w_before + (n - 1.) * w < goal_w)) n -= 1.;
-      while (w > 0. && w_before + n * w < goal_w) n += 1.;
-      cut.ties = n < 1. ? 1 : n > 1e9 ? 1000000000 : (int)n;
-    }
-    return cut;
-  };
-  // the weight of a beginning, the same in every thread; equals beyond the cut are told apart by number, not by index
-  const auto weigh = [&](const Cut& cut) {
+    if (by_count) return {prefix, prefix == sample_key(-INFINITY) ? 0 : goal_n - (int)before};  // (what is -inf has no weight)
+    // equals have one weight: the j-th (from 0) is kept where what stands before it is below the goal
+    const double w = (double)weight(sample_logit(prefix));
+    double n = w > 0. ? ceil((goal_w - before) / w) : 1.;
+    while (n > 1. && !(before + (n - 1.) * w < goal_w)) n -= 1.;
+    while (w > 0. && before + n * w < goal_w) n += 1.;
+    return {prefix, n < 1. ? 1 : n > 1e9 ? 1000000000 : (int)n};
+  }
+  // the weight of such a beginning, the same in every thread
+  __device__ __forceinline__ double weigh(const Weights& weight, const Digits& d) const {
     double sum = 0.;
     for (int v = tid; v < nv; v += SAMPLE_THREADS) {
       float l[E];
       x.load(v, l);
 #pragma unroll
       for (int e = 0; e < E; e++)
-        if (sample_key(l[e]) > cut.key) sum += (double)weight(l[e]);
+        if (sample_key(l[e]) > d.key) sum += (double)weight(l[e]);
     }
-    sum = wave_sum_f64(sum);
-    if (lane == 0) wd[wave] = sum;
-    __syncthreads();
-    sum = 0.;
-    for (int i = 0; i < SAMPLE_WAVES; i++) sum += wd[i];
-    __syncthreads();
-    return cut.ties ? sum + (double)cut.ties * (double)weight(sample_logit(cut.key)) : sum;
-  };
-
-  Cut cut{sample_key(-INFINITY), 0};  // all tokens above -inf
-  const int top_k = a.top_ks ? a.top_ks[row] : a.top_k;
-  const float top_p = fminf(fmaxf(a.top_ps ? a.top_ps[row] : a.top_p, 0.f), 1.f);
-  if (top_k > 0 && top_k < a.V) cut = find(true, top_k, 0.);
-  if (top_p < 1.f) {
-    const double goal = (double)top_p * weigh(cut);
-    if (goal > 0.) cut = find(false, 0, goal);
-    else cut = Cut{sample_key(m), 1};
+    double all;
+    group_scan(sum, s, all);
+    return d.ties ? all + (double)d.ties * (double)weight(sample_logit(d.key)) : all;
   }
   // where the cut goes through equals: the index of the first one left out
-  int end = 0x7fffffff;
-  if (cut.ties) {
-    int* here = reinterpret_cast<int*>(stretch);
-    for (int s = wave; s < stretches; s += SAMPLE_WAVES) {
-      const int v = s * WAVE + lane;
-      int n = 0;
-      if (v < nv) {
-        float l[E];
-        x.load(v, l);
+  __device__ __forceinline__ int end_of(const Digits& d) const {
+    if (!d.ties) return 0;
+    int* here = reinterpret_cast<int*>(s.mass);
+    visit([](int) { return true; },
+          [&](int c, int v, const float (&l)[E]) {
+            int n = 0;
 #pragma unroll
-        for (int e = 0; e < E; e++) n += sample_key(l[e]) == cut.key;
-      }
+            for (int e = 0; e < E; e++) n += sample_key(l[e]) == d.key;
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-      if (lane == 0) here[s] = n;
-    }
-    if (tid == 0) found_at = 0x7fffffff;
+            for (int o = SAMPLE_CELL / 2; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+            if (tid % SAMPLE_CELL == 0) here[c] = n;
+          });
+    if (tid == 0) s.at = 0x7fffffff;
     __syncthreads();
     if (tid == 0) {
-      int left = cut.ties;
-      for (int s = 0; s < stretches; s++) {
-        if (here[s] > left) {
-          for (int i = max(0, s * WAVE * E - x.lead); i < a.V; i++) {
-            const float l = Elem<T>::to_f(x.base[i + x.lead]);
-            if (sample_key(l) == cut.key && left-- == 0) {
-              found_at = i;
+      int left = d.ties;
+      for (int c = 0; c < cells; c++) {
+        if (here[c] > left) {
+          for (int i = max(0, x.index(c * SAMPLE_CELL, 0)); i < a.V; i++)
+            if (sample_key(Elem<T>::to_f(x.base[i + x.lead])) == d.key && left-- == 0) {
+              s.at = i;
               break;
             }
-          }
           break;
         }
-        left -= here[s];
+        left -= here[c];
       }
     }
     __syncthreads();
-    end = found_at;
+    const int end = s.at;
     __syncthreads();
+    return end;
   }
-  const float min_p = fminf(fmaxf(a.min_ps ? a.min_ps[row] : a.min_p, 0.f), 1.f);
-  // weight of token i with logit l in the draw: zero where it is not kept
-  const auto kept = [&](float l, int i) {
-    const unsigned key = sample_key(l);
-    const float w = weight(l);
-    return (key > cut.key || (key == cut.key && i < end && cut.ties)) && w >= min_p ? (double)w : 0.;
-  };
-  for (int s = wave; s < stretches; s += SAMPLE_WAVES) {
-    const int v = s * WAVE + lane;
-    double sum = 0.;
-    if (v < nv) {
-      float l[E];
-      x.load(v, l);
-#pragma unroll
-      for (int e = 0; e < E; e++) sum += kept(l[e], v * E + e - x.lead);
-    }
-    sum = wave_sum_f64(sum);
-    if (lane == 0) stretch[s] = sum;
+  __device__ __forceinline__ void by_digits(const Weights& weight) const {
+    Digits d{sample_key(-INFINITY), 0};  // all tokens above -inf
+    if (set.top_k) d = find(weight, true, set.top_k, 0.);
+    if (set.top_p < 1.f) d = find(weight, false, 0, (double)set.top_p * weigh(weight, d));
+    const int end = end_of(d);
+    const auto kept = [&](float l, int i) {
+      const unsigned key = sample_key(l);
+      const float w = weight(l);
+      return (key > d.key || (key == d.key && i < end)) && w >= set.min_p ? (double)w : 0.;
+    };
+    weigh_cells(kept);
+    draw_cells(kept);
   }
-  __syncthreads();
-  if (wave == 0) {
-    const int per = (stretches + 63) / 64;
-    double sum = 0.;
-    for (int i = 0; i < per && lane * per + i < stretches; i++) sum += stretch[lane * per + i];
-    double upto = sum;
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += y;
+};
+
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs a) {
+  __shared__ PickLds lds;
+  const Picker<T> p(a, lds);
+  constexpr int E = Picker<T>::E;
+  const Settings& set = p.set;
+  if (p.m == -INFINITY) {
+    if (p.tid == 0) {
+      a.tokens[p.row] = -1;
+      a.logprobs[p.row] = -INFINITY;
     }
-    const double all = __shfl(upto, 63, 64);
-    const float u = fminf(fmaxf(a.uniform[row], 0.f), 0x1.fffffep-1f);
-    const double goal = (double)u * all;
-    int l0 = __ffsll((unsigned long long)__ballot(upto > goal)) - 1;  // (all > goal)
-    double before = __shfl(upto - sum, l0, 64);
-    int s = l0 * per;
-    while (before + stretch[s] <= goal) before += stretch[s++];
-    // inside the stretch
-    const int v = s * WAVE + lane;
-    double w[E];
-    sum = 0.;
-    float l[E];
-    if (v < nv) x.load(v, l);
+    return;
+  }
+  if (set.kind == GREEDY) return p.greedy();
+  const Weights weight(p.m, set.temperature);
+  if (set.kind == DIGITS) return p.by_digits(weight);
+  if (set.kind == ALL) {
+    for (int c = p.tid; c < p.cells; c += SAMPLE_THREADS) lds.mass[c] = a.masses(p.row)[c];
+    __syncthreads();
+    return p.draw_cells([&](float l, int) { return (double)weight(l); });
+  }
+  if (set.kind == TOP_P) {
+    // the stretch of weights that the cut lies in
+    constexpr int PER = SAMPLE_BINS / SAMPLE_THREADS;
+    const double* bins = a.bins(p.row);
+    double w[PER], sum = 0., all;
 #pragma unroll
-    for (int e = 0; e < E; e++) sum += w[e] = v < nv ? kept(l[e], v * E + e - x.lead) : 0.;
-    upto = sum;
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(upto, o, 64);
-      if (lane >= o) upto += y;
-    }
-    l0 = __ffsll((unsigned long long)__ballot(before + upto > goal)) - 1;
-    if (lane == l0) {
-      before += upto - sum;
-      int e = 0;
+    for (int i = 0; i < PER; i++) sum += w[i] = bins[p.tid * PER + i];
+    const double upto = group_scan(sum, lds, all), goal = (double)set.top_p * all;
+    if (upto >= goal && upto - sum < goal) {
+      double begin = upto - sum;
+      int b = p.tid * PER;
 #pragma unroll
-      for (int i = 0; i < E - 1; i++)
-        if (e == i && before + w[i] <= goal) {
-          before += w[i];
-          e = i + 1;
+      for (int i = 0; i < PER - 1; i++)
+        if (b == p.tid * PER + i && begin + w[i] < goal) {
+          begin += w[i];
+          b++;
         }
-      double chosen = w[0];
-#pragma unroll
-      for (int i = 1; i < E; i++) chosen = e == i ? w[i] : chosen;
-      a.tokens[row] = v * E + e - x.lead;
-      a.logprobs[row] = (float)log(chosen / all);
+      lds.at = b;
+      lds.begin = begin;
     }
+    __syncthreads();
+    const int b = lds.at;
+    const double before = lds.begin;
+    // what ranks before it is kept; what lies in it goes to the list
+    p.visit([](int) { return true; },
+            [&](int c, int v, const float (&l)[E]) {
+              double cell = 0.;
+#pragma unroll
+              for (int e = 0; e < E; e++) {
+                const float x = weight.power(l[e]);
+                const int bin = Weights::bin(x);
+                if (bin > b) continue;
+                const float y = weight.of_power(x);
+                if (bin < b) cell += y >= set.min_p ? (double)y : 0.;
+                else if (y > 0.f) p.push(l[e], p.x.index(v, e));
+              }
+              cell = cell_sum(cell);
+              if (p.tid % SAMPLE_CELL == 0) lds.mass[c] = cell;
+            });
+    __syncthreads();
+    const int n = lds.count;
+    if (n > SAMPLE_LIST) return p.by_digits(weight);
+    sort_list(lds, n);
+    const uint64_t last = p.cut(weight, n, 0, before, goal);
+    if (p.tid < n && lds.list[p.tid] <= last) {
+      const float y = weight(p.listed(p.tid));
+      const int i = (int)(unsigned)lds.list[p.tid];
+      if (y >= set.min_p) atomicAdd(&lds.mass[(i + p.x.lead) / E / SAMPLE_CELL], (double)y);
+    }
+    __syncthreads();
+    return p.draw_cells([&](float l, int i) {
+      const float y = weight(l);
+      return ((uint64_t)~sample_key(l) << 32 | (unsigned)i) <= last && y >= set.min_p ? (double)y : 0.;
+    });
   }
+  // LIST, TOP_K, MIN_P: all that may be kept is listed
+  const float pivot = set.kind == TOP_K ? p.pivot(set.top_k) : -INFINITY, floor = set.kind == MIN_P ? set.min_p : 0.f;
+  // (a cell is looked into unless its largest weight is below min-p by more than the exponential's own error)
+  p.visit([&](int c) { return lds.maxima[c] > -INFINITY && lds.maxima[c] >= pivot && (floor == 0.f || weight(lds.maxima[c]) >= floor * 0.9999f); },
+          [&](int, int v, const float (&l)[E]) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+              if (l[e] > -INFINITY && l[e] >= pivot && (floor == 0.f || weight(l[e]) >= floor)) p.push(l[e], p.x.index(v, e));
+          });
+  __syncthreads();
+  const int n = lds.count;
+  if (n > SAMPLE_LIST) return p.by_digits(weight);
+  sort_list(lds, n);
+  p.draw_listed(weight, n, p.cut(weight, n, set.top_k, 0., -1.));
+}
+
+inline bool sample_needs_mass(const SampleArgs& a) {  // whether any row may, from what the host knows
+  const bool greedy = !a.temperatures && !(a.temperature > 0.f), top_k = !a.top_ks && a.top_k > 0 && a.top_k < a.V;
+  const bool min_p = !a.min_ps && a.min_p > 0.f && !a.top_ps && a.top_p >= 1.f;
+  return a.V > SAMPLE_LIST && !greedy && !top_k && !min_p;
+}
+
+template <typename T>
+void sample_launch(const SampleArgs& a, int B, hipStream_t st) {
+  constexpr int U = 4;
+  const int vectors = a.V / Row<T>::E + 2;
+  const dim3 grid((vectors + SAMPLE_SPLIT * U - 1) / (SAMPLE_SPLIT * U), B);
+  sample_cells_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
+  if (sample_needs_mass(a)) sample_mass_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
+  sample_pick_kernel<T><<<B, SAMPLE_THREADS, 0, st>>>(a);
 }
 
 }  // namespace tp
 
-extern "C" size_t tp_sample_workspace_bytes(int B, int V) { return 0; }
+extern "C" size_t tp_sample_workspace_bytes(int B, int V) {
+  using namespace tp;
+  return B < 1 || V < 1 || V > SAMPLE_MOST ? 0 : B * (size_t)SampleArgs::ws_row(sample_cells(V));
+}
 
 extern "C" int tp_sample(const void* logits, const float* uniform, const float* temperatures, const int32_t* top_ks, const float* top_ps,
                          const float* min_ps, float temperature, int top_k, float top_p, float min_p, int64_t* tokens, float* logprobs, void* ws,
@@ -350,12 +708,15 @@ extern "C" int tp_sample(const void* logits, const float* uniform, const float* 
   using namespace tp;
   TP_REQUIRE(logits && uniform && tokens && logprobs, TP_ERR_BAD_ARG, "tp_sample: null pointer");
   TP_REQUIRE(B >= 1 && V >= 1 && row_stride >= V, TP_ERR_BAD_ARG, "tp_sample: sizes must be positive and rows must not overlap");
-  TP_REQUIRE(V <= SAMPLE_MOST && B < (1 << 22), TP_ERR_UNSUPPORTED, "tp_sample: V=%d (at most 2^18), B=%d (below 2^22)", V, B);
+  TP_REQUIRE(V <= SAMPLE_MOST && B < (1 << 16), TP_ERR_UNSUPPORTED, "tp_sample: V=%d (at most 2^18), B=%d (below 2^16)", V, B);
   TP_REQUIRE(dtype >= TP_BF16 && dtype <= TP_F32, TP_ERR_UNSUPPORTED, "tp_sample: unsupported dtype code %d", dtype);
-  TP_REQUIRE(((uintptr_t)logits & (dtype == TP_F32 ? 3 : 1)) == 0, TP_ERR_BAD_ARG, "tp_sample: misaligned logits");
-  const SampleArgs a{logits, uniform, temperatures, top_ps, min_ps, top_ks, temperature, top_p, min_p, top_k, tokens, logprobs, row_stride, V};
-  if (dtype == TP_F32) sample_rows_kernel<float><<<B, SAMPLE_THREADS, 0, (hipStream_t)stream>>>(a);
-  else if (dtype == TP_BF16) sample_rows_kernel<bf16_t><<<B, SAMPLE_THREADS, 0, (hipStream_t)stream>>>(a);
-  else sample_rows_kernel<f16_t><<<B, SAMPLE_THREADS, 0, (hipStream_t)stream>>>(a);
+  TP_REQUIRE(((uintptr_t)logits & (dtype == TP_F32 ? 3 : 1)) == 0 && aligned16(ws), TP_ERR_BAD_ARG, "tp_sample: misaligned logits or workspace");
+  TP_REQUIRE(ws, TP_ERR_BAD_ARG, "tp_sample: no workspace");
+  const SampleArgs a{logits, uniform, temperatures, top_ps, min_ps, top_ks, temperature, top_p, min_p, top_k, tokens, logprobs, (char*)ws, row_stride, V,
+                     sample_cells(V)};
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == TP_F32) sample_launch<float>(a, B, st);
+  else if (dtype == TP_BF16) sample_launch<bf16_t>(a, B, st);
+  else sample_launch<f16_t>(a, B, st);
   return check_launch("tp_sample");
 }
