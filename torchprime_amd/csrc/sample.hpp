@@ -10,15 +10,17 @@
 // which its last token (logit, index) describes; min-p is a bound on the weight itself.  The draw walks the kept tokens by index,
 // which needs no sort of the row: a sum per cell of the row (16 vectors of 16 bytes), then the cell that the drawn weight falls into.
 //
-// Three launches, the second only where a row may need it:
+// Up to four launches, the two in the middle only where a row may need them:
 //   sample_cells_kernel  the row split over workgroups: the largest logit of each cell.  It reads everything, once, and is bound by HBM.
 //   sample_mass_kernel   rows without top-k: the weight of each cell (no filter at all), or of each of 2048 stretches of the logit's
 //                        range (top-p): the row again, from the caches unless the batch is larger than they are.
+//   sample_walk_kernel   top-p without top-k: the stretch that the cut lies in is known now; the weight of what ranks before it, cell by
+//                        cell, and a list of its tokens.
 //   sample_pick_kernel   a workgroup per row.  A short list of tokens decides: with top-k, those not below the k-th largest of the
-//                        cells' largest logits (at least k tokens are not), found in the few cells that hold any; with top-p, those of the
-//                        one stretch that the cut lies in, in one more walk over the row; with min-p, those that have the weight.  The list
-//                        is sorted by rank, cut, and drawn from.  Where it would not fit (thousands of equals, top-k in the
-//                        thousands), the cut is found digit by digit over an order-preserving integer key of the logits, slower.
+//                        cells' largest logits (at least k tokens are not), found in the few cells that hold any; with top-p, the list
+//                        above; with min-p, those that have the weight.  It is sorted by rank, cut, and drawn from.  Where it would not
+//                        fit (thousands of equals, top-k in the thousands), the cut is found digit by digit over an order-preserving
+//                        integer key of the logits, slower.
 #pragma once
 #include <float.h>
 
@@ -30,7 +32,7 @@ constexpr float SAMPLE_LOG2E = 1.4426950408889634f;
 constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / WAVE;
 constexpr int SAMPLE_MOST = 1 << 18;  // logits per row
 constexpr int SAMPLE_CELL = 16;       // vectors of 16 bytes, one per lane of a group of 16
-constexpr int SAMPLE_CELLS = SAMPLE_MOST / 4 / SAMPLE_CELL + 2;
+constexpr int SAMPLE_CELLS = SAMPLE_MOST / 4 / SAMPLE_CELL + 3;
 constexpr int SAMPLE_LIST = 1024;     // tokens that are sorted at most
 constexpr int SAMPLE_TOP_K = 640;     // the list takes top-k up to half the cells, and this: about C log(1 / (1 - k / C)) of C cells' tokens
 constexpr int SAMPLE_BINS = 2048;     // over weights from 1 down to 2^-36
@@ -47,14 +49,21 @@ struct SampleArgs {
   char* ws;
   int64_t row_stride;
   int V;
-  // of row r: the bins, the cells' weights, the cells' largest logits
-  static constexpr int64_t ws_row(int cells) { return (SAMPLE_BINS * 8 + (int64_t)cells * 12 + 15) / 16 * 16; }
-  int cells;
-  __device__ __forceinline__ double* bins(int r) const { return reinterpret_cast<double*>(ws + r * ws_row(cells)); }
-  __device__ __forceinline__ double* masses(int r) const { return bins(r) + SAMPLE_BINS; }
+  int cells;  // of any row, at most
+  // per row: what sample_walk_kernel found, its list, the bins, the cells' weights, the cells' largest logits
+  struct Walk {
+    double before, goal;
+    int bin, count;
+    int64_t none;
+  };
+  static constexpr int64_t ws_row(int cells) { return (sizeof(Walk) + SAMPLE_LIST * 8 + SAMPLE_BINS * 8 + (int64_t)cells * 12 + 15) / 16 * 16; }
+  __device__ __forceinline__ Walk* walk(int r) const { return reinterpret_cast<Walk*>(ws + r * ws_row(cells)); }
+  __device__ __forceinline__ uint64_t* list(int r) const { return reinterpret_cast<uint64_t*>(walk(r) + 1); }
+  __device__ __forceinline__ uint64_t* bins(int r) const { return list(r) + SAMPLE_LIST; }  // in units of 2^-35
+  __device__ __forceinline__ double* masses(int r) const { return reinterpret_cast<double*>(bins(r) + SAMPLE_BINS); }
   __device__ __forceinline__ float* maxima(int r) const { return reinterpret_cast<float*>(masses(r) + cells); }
 };
-inline int sample_cells(int V) { return (V / 4 + 2 + SAMPLE_CELL - 1) / SAMPLE_CELL; }  // at most, for any type and address
+inline int sample_cells(int V) { return (V / 4 + SAMPLE_CELL - 1) / SAMPLE_CELL + 2; }  // at most, for any type and address
 
 // larger logit, larger key; -0 and +0 have the same
 __device__ __forceinline__ unsigned sample_key(float l) {
@@ -72,6 +81,8 @@ struct Weights {
   __device__ __forceinline__ float power(float l) const { return l == m ? 0.f : (l - m) * c; }
   __device__ __forceinline__ float of_power(float x) const { return (__builtin_amdgcn_exp2f(x) + 0x1p-12f) - 0x1p-12f; }
   __device__ __forceinline__ float operator()(float l) const { return of_power(power(l)); }
+  // a weight in units of 2^-35: 2^17 + w has it in its last bits
+  __device__ __forceinline__ static uint64_t units(float w) { return __builtin_bit_cast(uint64_t, (double)w + 0x1p17) - __builtin_bit_cast(uint64_t, 0x1p17); }
   // falls as the logit rises; beyond the last bin nothing has a weight
   __device__ __forceinline__ static int bin(float x) { return (int)fminf(-x * SAMPLE_BIN, (float)SAMPLE_BINS); }
 };
@@ -95,30 +106,43 @@ struct Settings {
   }
 };
 
-// The logits of a row, 16 bytes at a time from 16-byte addresses; elements outside the row, and NaN, are -inf.
+// The logits of a row in vectors of 16 bytes at 16-byte addresses, and one cell each for the few elements before the first and
+// behind the last of them, one element a vector.  What is not there, and NaN, is -inf.
 template <typename T>
 struct Row {
   static constexpr int E = 16 / sizeof(T);
-  const T* base;  // 16-byte aligned, `lead` elements before the row's first
-  int lead, V;
-  __device__ __forceinline__ Row(const SampleArgs& a, int row) : V(a.V) {
-    const T* p = reinterpret_cast<const T*>(a.logits) + row * a.row_stride;
-    lead = (int)(((size_t)p & 15) / sizeof(T));
-    base = p - lead;
+  const T* p;
+  int head, full, padded;  // elements before the vectors; vectors; vectors up to a whole cell
+  int V;
+  __device__ __forceinline__ Row(const SampleArgs& a, int row) : p(reinterpret_cast<const T*>(a.logits) + row * a.row_stride), V(a.V) {
+    head = min(V, (int)((16 - ((size_t)p & 15)) % 16 / sizeof(T)));
+    full = (V - head) / E;
+    padded = (full + SAMPLE_CELL - 1) / SAMPLE_CELL * SAMPLE_CELL;
   }
-  __device__ __forceinline__ int vectors() const { return (V + lead + E - 1) / E; }
-  __device__ __forceinline__ int cells() const { return (vectors() + SAMPLE_CELL - 1) / SAMPLE_CELL; }
-  __device__ __forceinline__ int index(int vec, int e) const { return vec * E + e - lead; }
+  __device__ __forceinline__ int vectors() const { return padded + 2 * SAMPLE_CELL; }
+  __device__ __forceinline__ int cells() const { return padded / SAMPLE_CELL + 2; }
+  // of an element that is there
+  __device__ __forceinline__ int index(int vec, int e) const {
+    const int v = vec - SAMPLE_CELL;
+    return v < 0 ? vec : v < padded ? head + v * E + e : head + full * E + (v - padded);
+  }
+  __device__ __forceinline__ int cell_of(int i) const {
+    return i < head ? 0 : i < head + full * E ? 1 + (i - head) / (E * SAMPLE_CELL) : 1 + padded / SAMPLE_CELL;
+  }
   __device__ __forceinline__ void load(int vec, float (&x)[E]) const {
-    const int i0 = index(vec, 0);
-    if (i0 >= 0 && i0 + E <= V) {
-      load_f<T, E>(base + (int64_t)vec * E, x);
+    const int v = vec - SAMPLE_CELL;
+    if ((unsigned)v < (unsigned)full) {
+      load_f<T, E>(p + head + (int64_t)v * E, x);
+#pragma unroll
+      for (int e = 0; e < E; e++) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
     } else {
+      const int i = index(vec, 0);
+      const bool there = v < 0 ? vec < head : v >= padded && i < V;
 #pragma unroll
-      for (int e = 0; e < E; e++) x[e] = i0 + e >= 0 && i0 + e < V ? Elem<T>::to_f(base[(int64_t)vec * E + e]) : -INFINITY;
+      for (int e = 1; e < E; e++) x[e] = -INFINITY;
+      const float y = there ? Elem<T>::to_f(p[i]) : -INFINITY;
+      x[0] = y == y ? y : -INFINITY;
     }
-#pragma unroll
-    for (int e = 0; e < E; e++) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
   }
 };
 
@@ -159,13 +183,14 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a
     if (threadIdx.x % SAMPLE_CELL == 0 && v < nv) out[v / SAMPLE_CELL] = m;
   }
   // cleared for the next kernel to add to
-  for (int i = blockIdx.x * SAMPLE_SPLIT + threadIdx.x; i < SAMPLE_BINS; i += gridDim.x * SAMPLE_SPLIT) a.bins(row)[i] = 0.;
+  for (int i = blockIdx.x * SAMPLE_SPLIT + threadIdx.x; i < SAMPLE_BINS; i += gridDim.x * SAMPLE_SPLIT) a.bins(row)[i] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.walk(row)->count = 0;
 }
 
 template <typename T, int U>
 __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
-  __shared__ double bins[SAMPLE_BINS];
+  __shared__ uint64_t bins[SAMPLE_BINS];
   __shared__ float wm[SAMPLE_SPLIT / WAVE];
   const int row = blockIdx.y, tid = threadIdx.x;
   const Row<T> x(a, row);
@@ -177,7 +202,7 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a)
   for (int i = tid; i < cells; i += SAMPLE_SPLIT) m = fmaxf(m, maxima[i]);
   m = wave_max(m);
   if (tid % WAVE == 0) wm[tid / WAVE] = m;
-  for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT) bins[i] = 0.;
+  for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT) bins[i] = 0;
   __syncthreads();
   for (int i = 0; i < SAMPLE_SPLIT / WAVE; i++) m = fmaxf(m, wm[i]);
   const Weights weight(m, s.temperature);
@@ -191,7 +216,7 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a)
       for (int e = 0; e < E; e++) {
         const float p = weight.power(l[e]), w = weight.of_power(p);
         if (s.kind == ALL) sum += (double)w;
-        else if (w > 0.f) atomicAdd(&bins[Weights::bin(p)], (double)w);
+        else if (w > 0.f) atomicAdd((unsigned long long*)&bins[Weights::bin(p)], (unsigned long long)Weights::units(w));
       }
     }
     if (s.kind == ALL) {
@@ -201,9 +226,93 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a)
   }
   if (s.kind == ALL) return;
   __syncthreads();
-  double* out = a.bins(row);
+  uint64_t* out = a.bins(row);
   for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT)
-    if (bins[i] > 0.) __hip_atomic_fetch_add(&out[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // (exact, so in any order)
+    if (bins[i]) __hip_atomic_fetch_add(&out[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// larger logits, and lower indices among equals, first
+__device__ __forceinline__ uint64_t sample_rank(float l, int i) { return (uint64_t)~sample_key(l) << 32 | (unsigned)i; }
+
+template <typename T, int U>
+__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a) {
+  constexpr int E = Row<T>::E, WAVES = SAMPLE_SPLIT / WAVE, PER = SAMPLE_BINS / SAMPLE_SPLIT;
+  __shared__ double wd[WAVES], found[2];
+  __shared__ float wm[WAVES];
+  __shared__ int found_bin;
+  const int row = blockIdx.y, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
+  const Row<T> x(a, row);
+  const int nv = x.vectors(), cells = x.cells(), v0 = blockIdx.x * (SAMPLE_SPLIT * U) + tid;
+  const Settings s(a, row, cells);
+  if (s.kind != TOP_P) return;
+  float m = -INFINITY;
+  const float* maxima = a.maxima(row);
+  for (int i = tid; i < cells; i += SAMPLE_SPLIT) m = fmaxf(m, maxima[i]);
+  // the stretch of weights that the cut lies in
+  double w[PER], sum = 0.;
+#pragma unroll
+  for (int i = 0; i < PER; i++) sum += w[i] = (double)a.bins(row)[tid * PER + i] * 0x1p-35;
+  double upto = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += y;
+  }
+  m = wave_max(m);
+  if (lane == 0) wm[wave] = m;
+  if (lane == WAVE - 1) wd[wave] = upto;
+  __syncthreads();
+  double all = 0.;
+  for (int i = 0; i < WAVES; i++) {
+    m = fmaxf(m, wm[i]);
+    upto += i < wave ? wd[i] : 0.;
+    all += wd[i];
+  }
+  const double goal = (double)s.top_p * all;
+  if (upto >= goal && upto - sum < goal) {  // (one thread: the sums are exact, and goal is above 0)
+    double begin = upto - sum;
+    int b = tid * PER;
+#pragma unroll
+    for (int i = 0; i < PER - 1; i++)
+      if (b == tid * PER + i && begin + w[i] < goal) {
+        begin += w[i];
+        b++;
+      }
+    found_bin = b;
+    found[0] = begin;
+  }
+  __syncthreads();
+  const int b = found_bin;
+  SampleArgs::Walk* out = a.walk(row);
+  if (blockIdx.x == 0 && tid == 0) {
+    out->before = found[0];
+    out->goal = goal;
+    out->bin = b;
+  }
+  const Weights weight(m, s.temperature);
+  for (int u = 0; u < U; u++) {
+    const int v = v0 + u * SAMPLE_SPLIT;
+    double cell = 0.;
+    if (v < nv) {
+      float l[E];
+      x.load(v, l);
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const float p = weight.power(l[e]);
+        const int bin = Weights::bin(p);
+        if (bin > b) continue;
+        const float y = weight.of_power(p);
+        if (bin < b) {
+          cell += y >= s.min_p ? (double)y : 0.;
+        } else if (y > 0.f) {
+          const int at = __hip_atomic_fetch_add(&out->count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (at < SAMPLE_LIST) a.list(row)[at] = sample_rank(l[e], x.index(v, e));
+        }
+      }
+    }
+    cell = cell_sum(cell);
+    if (tid % SAMPLE_CELL == 0 && v < nv) a.masses(row)[v / SAMPLE_CELL] = cell;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -241,13 +350,31 @@ __device__ __forceinline__ double group_scan(double v, PickLds& s, double& all) 
 
 // list[0, n) in rising order; places from n to the next power of two are filled up
 __device__ __forceinline__ void sort_list(PickLds& s, int n) {
-  int size = 64;
+  if (n <= WAVE) {  // (the usual case: one wave, in its registers)
+    if (threadIdx.x < WAVE) {
+      const int lane = threadIdx.x;
+      uint64_t x = lane < n ? s.list[lane] : ~0ull;
+#pragma unroll
+      for (int k = 2; k <= WAVE; k *= 2)
+#pragma unroll
+        for (int j = k / 2; j > 0; j /= 2) {
+          const uint64_t y = __shfl_xor((unsigned long long)x, j, 64);
+          const bool lower = (lane & j) == 0, rising = (lane & k) == 0;
+          x = (lower == rising) == (x < y) ? x : y;
+        }
+      s.list[lane] = x;
+    }
+    __syncthreads();
+    return;
+  }
+  int size = 2 * WAVE;
   while (size < n) size *= 2;
   for (int i = n + threadIdx.x; i < size; i += SAMPLE_THREADS) s.list[i] = ~0ull;
   __syncthreads();
   for (int k = 2; k <= size; k *= 2)
     for (int j = k / 2; j > 0; j /= 2) {
-      for (int i = threadIdx.x; i < size / 2; i += SAMPLE_THREADS) {
+      const int i = threadIdx.x;
+      if (i < size / 2) {
         const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
         const uint64_t x = s.list[lo], y = s.list[hi];
         if ((x > y) == ((lo & k) == 0)) {
@@ -302,10 +429,7 @@ struct Picker {
       if (!wants(c)) continue;
       const int v = c * SAMPLE_CELL + tid % SAMPLE_CELL;
       float l[E];
-      if (v < nv) x.load(v, l);
-      else
-#pragma unroll
-        for (int e = 0; e < E; e++) l[e] = -INFINITY;
+      x.load(v, l);
       f(c, v, l);
     }
   }
@@ -325,7 +449,7 @@ struct Picker {
   // Tokens for the list, ranked: the inverted key above the index
   __device__ __forceinline__ void push(float l, int i) const {
     const int at = atomicAdd(&s.count, 1);
-    if (at < SAMPLE_LIST) s.list[at] = (uint64_t)~sample_key(l) << 32 | (unsigned)i;
+    if (at < SAMPLE_LIST) s.list[at] = sample_rank(l, i);
   }
   __device__ __forceinline__ float listed(int at) const { return sample_logit(~(unsigned)(s.list[at] >> 32)); }
 
@@ -429,9 +553,9 @@ struct Picker {
     float l[E];
     double token[E];
     sum = 0.;
-    if (v < nv) x.load(v, l);
+    x.load(v, l);
 #pragma unroll
-    for (int e = 0; e < E; e++) sum += token[e] = v < nv ? kept(l[e], x.index(v, e)) : 0.;
+    for (int e = 0; e < E; e++) sum += token[e] = kept(l[e], x.index(v, e));
     double here = sum;
 #pragma unroll
     for (int o = 1; o < SAMPLE_CELL; o <<= 1) {
@@ -557,8 +681,8 @@ struct Picker {
       int left = d.ties;
       for (int c = 0; c < cells; c++) {
         if (here[c] > left) {
-          for (int i = max(0, x.index(c * SAMPLE_CELL, 0)); i < a.V; i++)
-            if (sample_key(Elem<T>::to_f(x.base[i + x.lead])) == d.key && left-- == 0) {
+          for (int i = x.index(c * SAMPLE_CELL, 0); i < a.V; i++)
+            if (sample_key(Elem<T>::to_f(x.p[i])) == d.key && left-- == 0) {
               s.at = i;
               break;
             }
@@ -591,8 +715,8 @@ template <typename T>
 __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs a) {
   __shared__ PickLds lds;
   const Picker<T> p(a, lds);
-  constexpr int E = Picker<T>::E;
   const Settings& set = p.set;
+  constexpr int E = Picker<T>::E;
   if (p.m == -INFINITY) {
     if (p.tid == 0) {
       a.tokens[p.row] = -1;
@@ -609,58 +733,25 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
     return p.draw_cells([&](float l, int) { return (double)weight(l); });
   }
   if (set.kind == TOP_P) {
-    // the stretch of weights that the cut lies in
-    constexpr int PER = SAMPLE_BINS / SAMPLE_THREADS;
-    const double* bins = a.bins(p.row);
-    double w[PER], sum = 0., all;
-#pragma unroll
-    for (int i = 0; i < PER; i++) sum += w[i] = bins[p.tid * PER + i];
-    const double upto = group_scan(sum, lds, all), goal = (double)set.top_p * all;
-    if (upto >= goal && upto - sum < goal) {
-      double begin = upto - sum;
-      int b = p.tid * PER;
-#pragma unroll
-      for (int i = 0; i < PER - 1; i++)
-        if (b == p.tid * PER + i && begin + w[i] < goal) {
-          begin += w[i];
-          b++;
-        }
-      lds.at = b;
-      lds.begin = begin;
-    }
-    __syncthreads();
-    const int b = lds.at;
-    const double before = lds.begin;
-    // what ranks before it is kept; what lies in it goes to the list
-    p.visit([](int) { return true; },
-            [&](int c, int v, const float (&l)[E]) {
-              double cell = 0.;
-#pragma unroll
-              for (int e = 0; e < E; e++) {
-                const float x = weight.power(l[e]);
-                const int bin = Weights::bin(x);
-                if (bin > b) continue;
-                const float y = weight.of_power(x);
-                if (bin < b) cell += y >= set.min_p ? (double)y : 0.;
-                else if (y > 0.f) p.push(l[e], p.x.index(v, e));
-              }
-              cell = cell_sum(cell);
-              if (p.tid % SAMPLE_CELL == 0) lds.mass[c] = cell;
-            });
-    __syncthreads();
-    const int n = lds.count;
+    // what ranks before the cut's stretch has been weighed, what lies in it is on the list
+    const SampleArgs::Walk& walk = *a.walk(p.row);
+    const int n = walk.count;
+    const double before = walk.before, goal = walk.goal;
     if (n > SAMPLE_LIST) return p.by_digits(weight);
+    for (int c = p.tid; c < p.cells; c += SAMPLE_THREADS) lds.mass[c] = a.masses(p.row)[c];
+    if (p.tid < n) lds.list[p.tid] = a.list(p.row)[p.tid];
+    __syncthreads();
     sort_list(lds, n);
     const uint64_t last = p.cut(weight, n, 0, before, goal);
     if (p.tid < n && lds.list[p.tid] <= last) {
       const float y = weight(p.listed(p.tid));
       const int i = (int)(unsigned)lds.list[p.tid];
-      if (y >= set.min_p) atomicAdd(&lds.mass[(i + p.x.lead) / E / SAMPLE_CELL], (double)y);
+      if (y >= set.min_p) atomicAdd(&lds.mass[p.x.cell_of(i)], (double)y);
     }
     __syncthreads();
     return p.draw_cells([&](float l, int i) {
       const float y = weight(l);
-      return ((uint64_t)~sample_key(l) << 32 | (unsigned)i) <= last && y >= set.min_p ? (double)y : 0.;
+      return sample_rank(l, i) <= last && y >= set.min_p ? (double)y : 0.;
     });
   }
   // LIST, TOP_K, MIN_P: all that may be kept is listed
@@ -688,10 +779,13 @@ inline bool sample_needs_mass(const SampleArgs& a) {  // whether any row may, fr
 template <typename T>
 void sample_launch(const SampleArgs& a, int B, hipStream_t st) {
   constexpr int U = 4;
-  const int vectors = a.V / Row<T>::E + 2;
+  const int vectors = a.V / Row<T>::E + 3 * SAMPLE_CELL;
   const dim3 grid((vectors + SAMPLE_SPLIT * U - 1) / (SAMPLE_SPLIT * U), B);
   sample_cells_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
-  if (sample_needs_mass(a)) sample_mass_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
+  if (sample_needs_mass(a)) {
+    sample_mass_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
+    if (a.top_ps || a.top_p < 1.f) sample_walk_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
+  }
   sample_pick_kernel<T><<<B, SAMPLE_THREADS, 0, st>>>(a);
 }
 
