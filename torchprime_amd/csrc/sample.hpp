@@ -24,6 +24,8 @@
 #pragma once
 #include <float.h>
 
+#include <algorithm>
+
 #include "common.hpp"
 
 namespace tp {
@@ -59,8 +61,8 @@ struct SampleArgs {
   static constexpr int64_t ws_row(int cells) { return (sizeof(Walk) + SAMPLE_LIST * 8 + SAMPLE_BINS * 8 + (int64_t)cells * 12 + 15) / 16 * 16; }
   __device__ __forceinline__ Walk* walk(int r) const { return reinterpret_cast<Walk*>(ws + r * ws_row(cells)); }
   __device__ __forceinline__ uint64_t* list(int r) const { return reinterpret_cast<uint64_t*>(walk(r) + 1); }
-  __device__ __forceinline__ uint64_t* bins(int r) const { return list(r) + SAMPLE_LIST; }  // in units of 2^-35
-  __device__ __forceinline__ double* masses(int r) const { return reinterpret_cast<double*>(bins(r) + SAMPLE_BINS); }
+  __device__ __forceinline__ double* bins(int r) const { return reinterpret_cast<double*>(list(r) + SAMPLE_LIST); }
+  __device__ __forceinline__ double* masses(int r) const { return bins(r) + SAMPLE_BINS; }
   __device__ __forceinline__ float* maxima(int r) const { return reinterpret_cast<float*>(masses(r) + cells); }
 };
 inline int sample_cells(int V) { return (V / 4 + SAMPLE_CELL - 1) / SAMPLE_CELL + 2; }  // at most, for any type and address
@@ -81,8 +83,6 @@ struct Weights {
   __device__ __forceinline__ float power(float l) const { return l == m ? 0.f : (l - m) * c; }
   __device__ __forceinline__ float of_power(float x) const { return (__builtin_amdgcn_exp2f(x) + 0x1p-12f) - 0x1p-12f; }
   __device__ __forceinline__ float operator()(float l) const { return of_power(power(l)); }
-  // a weight in units of 2^-35: 2^17 + w has it in its last bits
-  __device__ __forceinline__ static uint64_t units(float w) { return __builtin_bit_cast(uint64_t, (double)w + 0x1p17) - __builtin_bit_cast(uint64_t, 0x1p17); }
   // falls as the logit rises; beyond the last bin nothing has a weight
   __device__ __forceinline__ static int bin(float x) { return (int)fminf(-x * SAMPLE_BIN, (float)SAMPLE_BINS); }
 };
@@ -158,6 +158,7 @@ __device__ __forceinline__ double cell_sum(double v) {
 }
 
 // ------------------------------------------------------------------------------------------------
+constexpr int SAMPLE_SHARES = 2048;  // workgroups of the second and third launch
 constexpr int SAMPLE_SPLIT = 256;  // threads of a workgroup that takes a part of a row
 template <typename T, int U>
 __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a) {
@@ -187,14 +188,29 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a
   if (blockIdx.x == 0 && threadIdx.x == 0) a.walk(row)->count = 0;
 }
 
-template <typename T, int U>
-__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a) {
+// f(vector, its logits) of every SAMPLE_SPLIT-th vector from v on, the loads four at a time
+template <typename T, typename F>
+__device__ __forceinline__ void each_vector(const Row<T>& x, int v, int end, F&& f) {
+  constexpr int E = Row<T>::E, U = 4;
+  for (; v < end; v += U * SAMPLE_SPLIT) {
+    float l[U][E];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (v + u * SAMPLE_SPLIT < end) x.load(v + u * SAMPLE_SPLIT, l[u]);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (v + u * SAMPLE_SPLIT < end) f(v + u * SAMPLE_SPLIT, l[u]);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a, int share) {
   constexpr int E = Row<T>::E;
-  __shared__ uint64_t bins[SAMPLE_BINS];
+  __shared__ double bins[SAMPLE_BINS];
   __shared__ float wm[SAMPLE_SPLIT / WAVE];
   const int row = blockIdx.y, tid = threadIdx.x;
   const Row<T> x(a, row);
-  const int nv = x.vectors(), cells = x.cells(), v0 = blockIdx.x * (SAMPLE_SPLIT * U) + tid;
+  const int cells = x.cells(), v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
   const Settings s(a, row, cells);
   if (s.kind != TOP_P && s.kind != ALL) return;
   float m = -INFINITY;
@@ -206,43 +222,38 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a)
   __syncthreads();
   for (int i = 0; i < SAMPLE_SPLIT / WAVE; i++) m = fmaxf(m, wm[i]);
   const Weights weight(m, s.temperature);
-  for (int u = 0; u < U; u++) {
-    const int v = v0 + u * SAMPLE_SPLIT;
+  each_vector(x, v0 + tid, v1, [&](int v, const float (&l)[E]) {  // (whole cells: shares and vectors() are multiples of 16)
     double sum = 0.;
-    if (v < nv) {
-      float l[E];
-      x.load(v, l);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float p = weight.power(l[e]), w = weight.of_power(p);
-        if (s.kind == ALL) sum += (double)w;
-        else if (w > 0.f) atomicAdd((unsigned long long*)&bins[Weights::bin(p)], (unsigned long long)Weights::units(w));
-      }
+    for (int e = 0; e < E; e++) {
+      const float p = weight.power(l[e]), w = weight.of_power(p);
+      if (s.kind == ALL) sum += (double)w;
+      else if (w > 0.f) atomicAdd(&bins[Weights::bin(p)], (double)w);
     }
     if (s.kind == ALL) {
       sum = cell_sum(sum);
-      if (tid % SAMPLE_CELL == 0 && v < nv) a.masses(row)[v / SAMPLE_CELL] = sum;
+      if (tid % SAMPLE_CELL == 0) a.masses(row)[v / SAMPLE_CELL] = sum;
     }
-  }
+  });
   if (s.kind == ALL) return;
   __syncthreads();
-  uint64_t* out = a.bins(row);
+  double* out = a.bins(row);
   for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT)
-    if (bins[i]) __hip_atomic_fetch_add(&out[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (bins[i] > 0.) __hip_atomic_fetch_add(&out[i], bins[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // larger logits, and lower indices among equals, first
 __device__ __forceinline__ uint64_t sample_rank(float l, int i) { return (uint64_t)~sample_key(l) << 32 | (unsigned)i; }
 
-template <typename T, int U>
-__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a) {
+template <typename T>
+__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a, int share) {
   constexpr int E = Row<T>::E, WAVES = SAMPLE_SPLIT / WAVE, PER = SAMPLE_BINS / SAMPLE_SPLIT;
   __shared__ double wd[WAVES], found[2];
   __shared__ float wm[WAVES];
   __shared__ int found_bin;
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
   const Row<T> x(a, row);
-  const int nv = x.vectors(), cells = x.cells(), v0 = blockIdx.x * (SAMPLE_SPLIT * U) + tid;
+  const int cells = x.cells(), v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
   const Settings s(a, row, cells);
   if (s.kind != TOP_P) return;
   float m = -INFINITY;
@@ -251,7 +262,7 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a)
   // the stretch of weights that the cut lies in
   double w[PER], sum = 0.;
 #pragma unroll
-  for (int i = 0; i < PER; i++) sum += w[i] = (double)a.bins(row)[tid * PER + i] * 0x1p-35;
+  for (int i = 0; i < PER; i++) sum += w[i] = a.bins(row)[tid * PER + i];
   double upto = sum;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -290,39 +301,36 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a)
     out->bin = b;
   }
   const Weights weight(m, s.temperature);
-  for (int u = 0; u < U; u++) {
-    const int v = v0 + u * SAMPLE_SPLIT;
+  each_vector(x, v0 + tid, v1, [&](int v, const float (&l)[E]) {
     double cell = 0.;
-    if (v < nv) {
-      float l[E];
-      x.load(v, l);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float p = weight.power(l[e]);
-        const int bin = Weights::bin(p);
-        if (bin > b) continue;
-        const float y = weight.of_power(p);
-        if (bin < b) {
-          cell += y >= s.min_p ? (double)y : 0.;
-        } else if (y > 0.f) {
-          const int at = __hip_atomic_fetch_add(&out->count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          if (at < SAMPLE_LIST) a.list(row)[at] = sample_rank(l[e], x.index(v, e));
-        }
+    for (int e = 0; e < E; e++) {
+      const float p = weight.power(l[e]);
+      const int bin = Weights::bin(p);
+      if (bin > b) continue;
+      const float y = weight.of_power(p);
+      if (bin < b) {
+        cell += y >= s.min_p ? (double)y : 0.;
+      } else if (y > 0.f) {
+        const int at = __hip_atomic_fetch_add(&out->count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (at < SAMPLE_LIST) a.list(row)[at] = sample_rank(l[e], x.index(v, e));
       }
     }
     cell = cell_sum(cell);
-    if (tid % SAMPLE_CELL == 0 && v < nv) a.masses(row)[v / SAMPLE_CELL] = cell;
-  }
+    if (tid % SAMPLE_CELL == 0) a.masses(row)[v / SAMPLE_CELL] = cell;
+  });
 }
 
 // ------------------------------------------------------------------------------------------------
 struct PickLds {
   double mass[SAMPLE_CELLS];
   float maxima[SAMPLE_CELLS];
+  unsigned short chosen[SAMPLE_CELLS];
   uint64_t list[SAMPLE_LIST];
   double wd[SAMPLE_WAVES];
-  float wf[SAMPLE_WAVES];
-  int count, at;
+  float most[SAMPLE_WAVES], least[SAMPLE_WAVES];
+  int wi[SAMPLE_WAVES];
+  int count, cells, at;
   double begin;
   uint64_t last;
 };
@@ -395,26 +403,37 @@ struct Picker {
   const Row<T> x;
   const int nv, cells;
   const Settings set;
-  float m;
+  float m, least, scale;  // of the cells' maxima, the largest and the smallest that is not -inf
 
   __device__ __forceinline__ Picker(const SampleArgs& args, PickLds& lds)
       : a(args), s(lds), row(blockIdx.x), tid(threadIdx.x), lane(tid & 63), wave(tid >> 6), x(args, blockIdx.x), nv(x.vectors()), cells(x.cells()),
         set(args, blockIdx.x, cells) {
     m = -INFINITY;
+    least = INFINITY;
     const float* maxima = a.maxima(row);
     for (int i = tid; i < cells; i += SAMPLE_THREADS) {
       const float c = maxima[i];
       s.maxima[i] = c;
       m = fmaxf(m, c);
+      least = fminf(least, c > -INFINITY ? c : INFINITY);
     }
     m = wave_max(m);
-    if (lane == 0) s.wf[wave] = m;
+    least = -wave_max(-least);
+    if (lane == 0) {
+      s.most[wave] = m;
+      s.least[wave] = least;
+    }
     if (tid == 0) {
-      s.count = 0;
+      s.count = s.cells = 0;
       s.at = 0x7fffffff;
     }
+    reinterpret_cast<int*>(s.mass)[tid] = 0;  // (the counts of pivot)
     __syncthreads();
-    for (int i = 0; i < SAMPLE_WAVES; i++) m = fmaxf(m, s.wf[i]);
+    for (int i = 0; i < SAMPLE_WAVES; i++) {
+      m = fmaxf(m, s.most[i]);
+      least = fminf(least, s.least[i]);
+    }
+    scale = 1023.f / (m - least);
   }
 
   __device__ __forceinline__ void answer(int token, double chosen, double all) const {
@@ -422,11 +441,11 @@ struct Picker {
     a.logprobs[row] = (float)log(chosen / all);
   }
 
-  // f(vector, its logits) of the cells that `wants`; every lane of a cell's 16 together
-  template <typename W, typename F>
-  __device__ __forceinline__ void visit(W&& wants, F&& f) const {
-    for (int c = tid / SAMPLE_CELL; c < cells; c += SAMPLE_THREADS / SAMPLE_CELL) {
-      if (!wants(c)) continue;
+  // f(cell, vector, its logits), every lane of a cell's 16 together: of all cells, or of the `n` chosen ones
+  template <typename F>
+  __device__ __forceinline__ void visit(F&& f, int n = -1) const {
+    for (int i = tid / SAMPLE_CELL; i < (n < 0 ? cells : n); i += SAMPLE_THREADS / SAMPLE_CELL) {
+      const int c = n < 0 ? i : s.chosen[i];
       const int v = c * SAMPLE_CELL + tid % SAMPLE_CELL;
       float l[E];
       x.load(v, l);
@@ -434,14 +453,23 @@ struct Picker {
     }
   }
 
+  // the cells that `wants`, in any order, and how many
+  template <typename W>
+  __device__ __forceinline__ int choose(W&& wants) const {
+    for (int c = tid; c < cells; c += SAMPLE_THREADS)
+      if (wants(s.maxima[c])) s.chosen[atomicAdd(&s.cells, 1)] = (unsigned short)c;
+    __syncthreads();
+    return s.cells;
+  }
+
   // the first index of the largest logit
   __device__ __forceinline__ void greedy() const {
-    visit([&](int c) { return s.maxima[c] == m; },
-          [&](int, int v, const float (&l)[E]) {
+    const int n = choose([&](float l) { return l == m; });
+    visit([&](int, int v, const float (&l)[E]) {
 #pragma unroll
-            for (int e = 0; e < E; e++)
-              if (l[e] == m) atomicMin(&s.at, x.index(v, e));
-          });
+      for (int e = 0; e < E; e++)
+        if (l[e] == m) atomicMin(&s.at, x.index(v, e));
+    }, n);
     __syncthreads();
     if (tid == 0) answer(s.at, 1., 1.);
   }
@@ -453,39 +481,29 @@ struct Picker {
   }
   __device__ __forceinline__ float listed(int at) const { return sample_logit(~(unsigned)(s.list[at] >> 32)); }
 
-  // a logit that at least k tokens reach: not above the k-th largest of the cells' maxima, in steps of 1/1024 of their range
+  // A bound that at least k tokens reach: the k-th largest of the cells' maxima, rounded down to 1/1023 of their range.  A logit
+  // reaches it where !(scaled(l) < bound); that is monotone in l, and true for the largest whatever the range is.
+  __device__ __forceinline__ float scaled(float l) const { return (l - least) * scale; }
   __device__ __forceinline__ float pivot(int k) const {
-    int* hist = reinterpret_cast<int*>(s.mass);
-    float lo = INFINITY;
+    static_assert(SAMPLE_THREADS == 1024, "a thread per step");
+    int* counts = reinterpret_cast<int*>(s.mass);
     for (int i = tid; i < cells; i += SAMPLE_THREADS)
-      if (s.maxima[i] > -INFINITY) lo = fminf(lo, s.maxima[i]);
-    lo = -wave_max(-lo);
-    for (int i = tid; i < 1024; i += SAMPLE_THREADS) hist[i] = 0;
-    __syncthreads();  // (the maxima's reduction has been read)
-    if (lane == 0) s.wf[wave] = lo;
+      if (s.maxima[i] > -INFINITY) atomicAdd(&counts[1023 - max(0, min(1023, (int)scaled(s.maxima[i])))], 1);
     __syncthreads();
-    for (int i = 0; i < SAMPLE_WAVES; i++) lo = fminf(lo, s.wf[i]);
-    const float step = (m - lo) * (1.f / 1023.f);
-    const auto bin = [&](float l) { return step > 0.f && step < INFINITY ? 1023 - min(1023, (int)((l - lo) / step)) : 0; };
-    for (int i = tid; i < cells; i += SAMPLE_THREADS)
-      if (s.maxima[i] > -INFINITY) atomicAdd(&hist[bin(s.maxima[i])], 1);
+    const int n = counts[tid];
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += y;
+    }
+    if (lane == 63) s.wi[wave] = upto;
     __syncthreads();
-    // (cells with anything in them may be fewer than k: then the pivot is the smallest, and the list may come out too long)
-    double all;
-    const double n = tid < 1024 ? (double)hist[tid] : 0., upto = group_scan(n, s, all);
-    if (upto >= k && upto - n < k) s.at = tid;
+    for (int i = 0; i < wave; i++) upto += s.wi[i];
+    if (upto >= k && upto - n < k) s.at = 1023 - tid;
     __syncthreads();
-    const int b = s.at;
-    float p = m;
-    if (all < k) p = -INFINITY;
-    else
-      for (int i = tid; i < cells; i += SAMPLE_THREADS)
-        if (s.maxima[i] > -INFINITY && bin(s.maxima[i]) <= b) p = fminf(p, s.maxima[i]);
-    p = -wave_max(-p);
-    if (lane == 0) s.wf[wave] = p;
-    __syncthreads();
-    for (int i = 0; i < SAMPLE_WAVES; i++) p = fminf(p, s.wf[i]);
-    return p;
+    // (cells with anything in them may be fewer than k: then all tokens are taken, and the list may come out too long)
+    return s.at > 1023 ? -INFINITY : (float)s.at;
   }
 
   // Of the sorted list, behind tokens of weight `before`: the last token kept by top-k and top-p (goal < 0: of the list's own weight)
@@ -501,6 +519,38 @@ struct Picker {
     if (kept && !next) s.last = s.list[tid];
     __syncthreads();
     return s.last;
+  }
+
+  // The same cut and draw of up to 64 unsorted tokens by one wave: a lane adds up what ranks before its token, then what is kept and
+  // comes before it by index, taking all tokens in turn.
+  __device__ __forceinline__ void draw_few(const Weights& weight, int n, int k) const {
+    const uint64_t token = lane < n ? s.list[lane] : ~0ull;
+    const float y = lane < n ? weight(listed(lane)) : 0.f;
+    const double w = (double)y;
+    const auto of_lane = [](double v, int i) {
+      const uint64_t u = __builtin_bit_cast(uint64_t, v);
+      return __builtin_bit_cast(double, (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(u >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)u, i));
+    };
+    int rank = 0;
+    double before = 0.;
+    for (int i = 0; i < n; i++) {
+      const uint64_t other = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(token >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)token, i);
+      const double v = of_lane(w, i);
+      rank += other < token;
+      before += other < token ? v : 0.;
+    }
+    const bool in = lane < n && (k == 0 || rank < k);
+    const double all = wave_sum_f64(in ? w : 0.), goal = set.top_p < 1.f ? (double)set.top_p * all : INFINITY;
+    const double kept = in && (rank == 0 || before < goal) && y >= set.min_p ? w : 0.;
+    const int index = (int)(unsigned)token;
+    double upto = kept, mass = 0.;
+    for (int i = 0; i < n; i++) {
+      const double v = of_lane(kept, i);
+      upto += __builtin_amdgcn_readlane(index, i) < index ? v : 0.;
+      mass += v;
+    }
+    const double drawn = (double)fminf(fmaxf(a.uniform[row], 0.f), 0x1.fffffep-1f) * mass;
+    if (kept > 0. && upto > drawn && upto - kept <= drawn) answer(index, kept, mass);
   }
 
   // Draws from the list (`n` sorted by rank, those up to `last` kept)
@@ -522,9 +572,13 @@ struct Picker {
     if (w > 0. && upto > goal && upto - w <= goal) answer((int)(s.list[tid] >> 32), w, all);
   }
 
-  // Draws from the whole row: cells' weights in s.mass, kept(l, i) a token's weight
-  template <typename K>
-  __device__ __forceinline__ void draw_cells(K&& kept) const {
+  // The weight in the draw of a token of the row, of which those that rank up to `last` are kept
+  __device__ __forceinline__ double kept(const Weights& weight, float l, int i, uint64_t last) const {
+    const float w = weight(l);
+    return sample_rank(l, i) <= last && w >= set.min_p ? (double)w : 0.;
+  }
+  // Draws from the whole row, the cells' weights in s.mass
+  __device__ __forceinline__ void draw_cells(const Weights& weight, uint64_t last) const {
     constexpr int PER = (SAMPLE_CELLS + SAMPLE_THREADS - 1) / SAMPLE_THREADS;
     double w[PER], sum = 0., all;
 #pragma unroll
@@ -555,7 +609,7 @@ struct Picker {
     sum = 0.;
     x.load(v, l);
 #pragma unroll
-    for (int e = 0; e < E; e++) sum += token[e] = kept(l[e], x.index(v, e));
+    for (int e = 0; e < E; e++) sum += token[e] = l[e] > -INFINITY ? kept(weight, l[e], x.index(v, e), last) : 0.;
     double here = sum;
 #pragma unroll
     for (int o = 1; o < SAMPLE_CELL; o <<= 1) {
@@ -569,20 +623,6 @@ struct Picker {
       if (left <= goal && left + token[e] > goal) answer(x.index(v, e), token[e], all);
       left += token[e];
     }
-  }
-
-  // The weight of kept(l, i) in every cell
-  template <typename K>
-  __device__ __forceinline__ void weigh_cells(K&& kept) const {
-    visit([](int) { return true; },
-          [&](int c, int v, const float (&l)[E]) {
-            double sum = 0.;
-#pragma unroll
-            for (int e = 0; e < E; e++) sum += kept(l[e], x.index(v, e));
-            sum = cell_sum(sum);
-            if (tid % SAMPLE_CELL == 0) s.mass[c] = sum;
-          });
-    __syncthreads();
   }
 
   // ---- the cut by digits, over the whole row ----
@@ -666,8 +706,7 @@ struct Picker {
   __device__ __forceinline__ int end_of(const Digits& d) const {
     if (!d.ties) return 0;
     int* here = reinterpret_cast<int*>(s.mass);
-    visit([](int) { return true; },
-          [&](int c, int v, const float (&l)[E]) {
+    visit([&](int c, int v, const float (&l)[E]) {
             int n = 0;
 #pragma unroll
             for (int e = 0; e < E; e++) n += sample_key(l[e]) == d.key;
@@ -696,18 +735,24 @@ struct Picker {
     __syncthreads();
     return end;
   }
-  __device__ __forceinline__ void by_digits(const Weights& weight) const {
+  // the last token kept; weighs the cells
+  __device__ __forceinline__ uint64_t by_digits(const Weights& weight) const {
     Digits d{sample_key(-INFINITY), 0};  // all tokens above -inf
-    if (set.top_k) d = find(weight, true, set.top_k, 0.);
-    if (set.top_p < 1.f) d = find(weight, false, 0, (double)set.top_p * weigh(weight, d));
-    const int end = end_of(d);
-    const auto kept = [&](float l, int i) {
-      const unsigned key = sample_key(l);
-      const float w = weight(l);
-      return (key > d.key || (key == d.key && i < end)) && w >= set.min_p ? (double)w : 0.;
-    };
-    weigh_cells(kept);
-    draw_cells(kept);
+    for (int by = 0; by < 2; by++) {
+      if (by == 0 ? set.top_k == 0 : !(set.top_p < 1.f)) continue;
+      const double goal = by == 0 ? 0. : (double)set.top_p * weigh(weight, d);
+      d = find(weight, by == 0, set.top_k, goal);
+    }
+    const uint64_t last = ((uint64_t)~d.key << 32) + (int64_t)end_of(d) - 1;
+    visit([&](int c, int v, const float (&l)[E]) {
+            double sum = 0.;
+#pragma unroll
+            for (int e = 0; e < E; e++) sum += l[e] > -INFINITY ? kept(weight, l[e], x.index(v, e), last) : 0.;
+            sum = cell_sum(sum);
+            if (tid % SAMPLE_CELL == 0) s.mass[c] = sum;
+          });
+    __syncthreads();
+    return last;
   }
 };
 
@@ -726,48 +771,52 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
   }
   if (set.kind == GREEDY) return p.greedy();
   const Weights weight(p.m, set.temperature);
-  if (set.kind == DIGITS) return p.by_digits(weight);
-  if (set.kind == ALL) {
-    for (int c = p.tid; c < p.cells; c += SAMPLE_THREADS) lds.mass[c] = a.masses(p.row)[c];
+  uint64_t last = ~0ull;
+  bool digits = set.kind == DIGITS;
+  if (set.kind == LIST || set.kind == TOP_K || set.kind == MIN_P) {
+    // all that may be kept is listed (a cell is looked into unless its largest weight is below min-p by more than the exponential's
+    // own error)
+    const float bound = set.kind == TOP_K ? p.pivot(set.top_k) : -INFINITY, floor = set.kind == MIN_P ? set.min_p : 0.f;
+    const int cells = p.choose([&](float l) { return l > -INFINITY && !(p.scaled(l) < bound) && (floor == 0.f || weight(l) >= floor * 0.9999f); });
+    p.visit([&](int, int v, const float (&l)[E]) {
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (l[e] > -INFINITY && !(p.scaled(l[e]) < bound) && (floor == 0.f || weight(l[e]) >= floor)) p.push(l[e], p.x.index(v, e));
+    }, cells);
     __syncthreads();
-    return p.draw_cells([&](float l, int) { return (double)weight(l); });
+    const int n = lds.count;
+    if (n <= WAVE) {
+      if (p.wave == 0) p.draw_few(weight, n, set.top_k);
+      return;
+    }
+    if (n <= SAMPLE_LIST) {
+      sort_list(lds, n);
+      return p.draw_listed(weight, n, p.cut(weight, n, set.top_k, 0., -1.));
+    }
+    digits = true;
   }
   if (set.kind == TOP_P) {
     // what ranks before the cut's stretch has been weighed, what lies in it is on the list
     const SampleArgs::Walk& walk = *a.walk(p.row);
     const int n = walk.count;
-    const double before = walk.before, goal = walk.goal;
-    if (n > SAMPLE_LIST) return p.by_digits(weight);
-    for (int c = p.tid; c < p.cells; c += SAMPLE_THREADS) lds.mass[c] = a.masses(p.row)[c];
-    if (p.tid < n) lds.list[p.tid] = a.list(p.row)[p.tid];
-    __syncthreads();
-    sort_list(lds, n);
-    const uint64_t last = p.cut(weight, n, 0, before, goal);
-    if (p.tid < n && lds.list[p.tid] <= last) {
-      const float y = weight(p.listed(p.tid));
-      const int i = (int)(unsigned)lds.list[p.tid];
-      if (y >= set.min_p) atomicAdd(&lds.mass[p.x.cell_of(i)], (double)y);
+    digits = n > SAMPLE_LIST;
+    if (!digits) {
+      for (int c = p.tid; c < p.cells; c += SAMPLE_THREADS) lds.mass[c] = a.masses(p.row)[c];
+      if (p.tid < n) lds.list[p.tid] = a.list(p.row)[p.tid];
+      __syncthreads();
+      sort_list(lds, n);
+      last = p.cut(weight, n, 0, walk.before, walk.goal);
+      if (p.tid < n && lds.list[p.tid] <= last) {
+        const float y = weight(p.listed(p.tid));
+        if (y >= set.min_p) atomicAdd(&lds.mass[p.x.cell_of((int)(unsigned)lds.list[p.tid])], (double)y);
+      }
     }
-    __syncthreads();
-    return p.draw_cells([&](float l, int i) {
-      const float y = weight(l);
-      return sample_rank(l, i) <= last && y >= set.min_p ? (double)y : 0.;
-    });
   }
-  // LIST, TOP_K, MIN_P: all that may be kept is listed
-  const float pivot = set.kind == TOP_K ? p.pivot(set.top_k) : -INFINITY, floor = set.kind == MIN_P ? set.min_p : 0.f;
-  // (a cell is looked into unless its largest weight is below min-p by more than the exponential's own error)
-  p.visit([&](int c) { return lds.maxima[c] > -INFINITY && lds.maxima[c] >= pivot && (floor == 0.f || weight(lds.maxima[c]) >= floor * 0.9999f); },
-          [&](int, int v, const float (&l)[E]) {
-#pragma unroll
-            for (int e = 0; e < E; e++)
-              if (l[e] > -INFINITY && l[e] >= pivot && (floor == 0.f || weight(l[e]) >= floor)) p.push(l[e], p.x.index(v, e));
-          });
+  if (set.kind == ALL)
+    for (int c = p.tid; c < p.cells; c += SAMPLE_THREADS) lds.mass[c] = a.masses(p.row)[c];
   __syncthreads();
-  const int n = lds.count;
-  if (n > SAMPLE_LIST) return p.by_digits(weight);
-  sort_list(lds, n);
-  p.draw_listed(weight, n, p.cut(weight, n, set.top_k, 0., -1.));
+  if (digits) last = p.by_digits(weight);
+  p.draw_cells(weight, last);
 }
 
 inline bool sample_needs_mass(const SampleArgs& a) {  // whether any row may, from what the host knows
@@ -783,8 +832,10 @@ void sample_launch(const SampleArgs& a, int B, hipStream_t st) {
   const dim3 grid((vectors + SAMPLE_SPLIT * U - 1) / (SAMPLE_SPLIT * U), B);
   sample_cells_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
   if (sample_needs_mass(a)) {
-    sample_mass_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
-    if (a.top_ps || a.top_p < 1.f) sample_walk_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
+    // (a share's fixed work - the cells' maxima, the bins - is that of some thousand logits: no more shares than fill the CUs)
+    const int parts = std::max(1, std::min((int)grid.x, SAMPLE_SHARES / B)), share = ((vectors + parts - 1) / parts + SAMPLE_CELL - 1) / SAMPLE_CELL * SAMPLE_CELL;
+    sample_mass_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share);
+    if (a.top_ps || a.top_p < 1.f) sample_walk_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share);
   }
   sample_pick_kernel<T><<<B, SAMPLE_THREADS, 0, st>>>(a);
 }
