@@ -151,11 +151,16 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-__device__ __forceinline__ double cell_sum(double v) {
-#pragma unroll
-  for (int o = SAMPLE_CELL / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+// over the 16 lanes of a cell, in the vector units (an exchange through LDS for every vector took as long as its arithmetic)
+template <int N> __device__ __forceinline__ int rotate16(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false); }
+template <int N> __device__ __forceinline__ double rotated_sum(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint64_t r = (uint64_t)(unsigned)rotate16<N>((int)(u >> 32)) << 32 | (unsigned)rotate16<N>((int)u);
+  return v + __builtin_bit_cast(double, r);
 }
+template <int N> __device__ __forceinline__ float rotated_max(float v) { return fmaxf(v, __int_as_float(rotate16<N>(__float_as_int(v)))); }
+__device__ __forceinline__ double cell_sum(double v) { return rotated_sum<1>(rotated_sum<2>(rotated_sum<4>(rotated_sum<8>(v)))); }
+__device__ __forceinline__ float cell_max(float v) { return rotated_max<1>(rotated_max<2>(rotated_max<4>(rotated_max<8>(v)))); }
 
 // ------------------------------------------------------------------------------------------------
 constexpr int SAMPLE_SHARES = 2048;  // workgroups of the second and third launch
@@ -179,8 +184,7 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a
 #pragma unroll
       for (int e = 0; e < E; e++) m = fmaxf(m, l[u][e]);
     }
-#pragma unroll
-    for (int o = SAMPLE_CELL / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    m = cell_max(m);
     if (threadIdx.x % SAMPLE_CELL == 0 && v < nv) out[v / SAMPLE_CELL] = m;
   }
   // cleared for the next kernel to add to
@@ -248,9 +252,10 @@ __device__ __forceinline__ uint64_t sample_rank(float l, int i) { return (uint64
 template <typename T>
 __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a, int share) {
   constexpr int E = Row<T>::E, WAVES = SAMPLE_SPLIT / WAVE, PER = SAMPLE_BINS / SAMPLE_SPLIT;
-  __shared__ double wd[WAVES], found[2];
+  __shared__ double wd[WAVES], found;
+  __shared__ uint64_t list[SAMPLE_LIST];
   __shared__ float wm[WAVES];
-  __shared__ int found_bin;
+  __shared__ int found_bin, count, begin_at;
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
   const Row<T> x(a, row);
   const int cells = x.cells(), v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
@@ -271,6 +276,7 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a,
   }
   m = wave_max(m);
   if (lane == 0) wm[wave] = m;
+  if (tid == 0) count = 0;
   if (lane == WAVE - 1) wd[wave] = upto;
   __syncthreads();
   double all = 0.;
@@ -290,13 +296,13 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a,
         b++;
       }
     found_bin = b;
-    found[0] = begin;
+    found = begin;
   }
   __syncthreads();
   const int b = found_bin;
   SampleArgs::Walk* out = a.walk(row);
   if (blockIdx.x == 0 && tid == 0) {
-    out->before = found[0];
+    out->before = found;
     out->goal = goal;
     out->bin = b;
   }
@@ -312,13 +318,20 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a,
       if (bin < b) {
         cell += y >= s.min_p ? (double)y : 0.;
       } else if (y > 0.f) {
-        const int at = __hip_atomic_fetch_add(&out->count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (at < SAMPLE_LIST) a.list(row)[at] = sample_rank(l[e], x.index(v, e));
+        const int at = atomicAdd(&count, 1);
+        if (at < SAMPLE_LIST) list[at] = sample_rank(l[e], x.index(v, e));
       }
     }
     cell = cell_sum(cell);
     if (tid % SAMPLE_CELL == 0) a.masses(row)[v / SAMPLE_CELL] = cell;
   });
+  // the workgroups' lists one behind the other, in the order that they come (the row's list is sorted later); beyond the list's end
+  // only the count goes on
+  __syncthreads();
+  if (tid == 0 && count) begin_at = __hip_atomic_fetch_add(&out->count, count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  for (int i = tid; i < min(count, SAMPLE_LIST); i += SAMPLE_SPLIT)
+    if (begin_at + i < SAMPLE_LIST) a.list(row)[begin_at + i] = list[i];
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -827,13 +840,17 @@ inline bool sample_needs_mass(const SampleArgs& a) {  // whether any row may, fr
 
 template <typename T>
 void sample_launch(const SampleArgs& a, int B, hipStream_t st) {
-  constexpr int U = 4;
+  // vectors a thread; us, one row of 128256 fp32, 256 rows: 2 14.3, 38.4; 4 15.1, 39.9; 8 16.6, 41.7
+  constexpr int U = 2;
   const int vectors = a.V / Row<T>::E + 3 * SAMPLE_CELL;
   const dim3 grid((vectors + SAMPLE_SPLIT * U - 1) / (SAMPLE_SPLIT * U), B);
   sample_cells_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
   if (sample_needs_mass(a)) {
-    // (a share's fixed work - the cells' maxima, the bins - is that of some thousand logits: no more shares than fill the CUs)
-    const int parts = std::max(1, std::min((int)grid.x, SAMPLE_SHARES / B)), share = ((vectors + parts - 1) / parts + SAMPLE_CELL - 1) / SAMPLE_CELL * SAMPLE_CELL;
+    // a share's fixed work - the cells' maxima, the bins - is that of some thousand logits, so no more shares than fill the CUs; twice as
+    // many where the settings are the rows' own, since only some rows need this then.  256 rows, 2048 : 4096, us: all with top-p 119 : 135,
+    // settings of their own 90 : 84
+    const int shares = SAMPLE_SHARES * (a.top_ks || a.top_ps || a.temperatures ? 2 : 1);
+    const int parts = std::max(1, std::min((vectors + 4 * SAMPLE_SPLIT - 1) / (4 * SAMPLE_SPLIT), shares / B)), share = ((vectors + parts - 1) / parts + SAMPLE_CELL - 1) / SAMPLE_CELL * SAMPLE_CELL;
     sample_mass_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share);
     if (a.top_ps || a.top_p < 1.f) sample_walk_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share);
   }
