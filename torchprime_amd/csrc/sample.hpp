@@ -35,6 +35,9 @@ constexpr int SAMPLE_THREADS = 1024, SAMPLE_WAVES = SAMPLE_THREADS / WAVE;
 constexpr int SAMPLE_MOST = 1 << 18;  // logits per row
 constexpr int SAMPLE_CELL = 16;       // vectors of 16 bytes, one per lane of a group of 16
 constexpr int SAMPLE_CELLS = SAMPLE_MOST / 4 / SAMPLE_CELL + 3;
+constexpr int SAMPLE_SPLIT = 256;     // threads of a workgroup that takes a part of a row
+constexpr int SAMPLE_FIRST = 2;       // vectors per thread of the first launch
+constexpr int SAMPLE_PARTS = SAMPLE_CELLS * SAMPLE_CELL / (SAMPLE_SPLIT * SAMPLE_FIRST) + 1;
 constexpr int SAMPLE_LIST = 1024;     // tokens that are sorted at most
 constexpr int SAMPLE_TOP_K = 640;     // the list takes top-k up to half the cells, and this: about C log(1 / (1 - k / C)) of C cells' tokens
 constexpr int SAMPLE_BINS = 2048;     // over weights from 1 down to 2^-36
@@ -52,18 +55,20 @@ struct SampleArgs {
   int64_t row_stride;
   int V;
   int cells;  // of any row, at most
-  // per row: what sample_walk_kernel found, its list, the bins, the cells' weights, the cells' largest logits
+  // per row: what sample_walk_kernel found, its list, the bins, the cells' weights, the largest logits of the first launch's workgroups
+  // and of the cells
   struct Walk {
     double before, goal;
     int bin, count;
     int64_t none;
   };
-  static constexpr int64_t ws_row(int cells) { return (sizeof(Walk) + SAMPLE_LIST * 8 + SAMPLE_BINS * 8 + (int64_t)cells * 12 + 15) / 16 * 16; }
+  static constexpr int64_t ws_row(int cells) { return (sizeof(Walk) + SAMPLE_LIST * 8 + SAMPLE_BINS * 8 + SAMPLE_PARTS * 4 + (int64_t)cells * 12 + 15) / 16 * 16; }
   __device__ __forceinline__ Walk* walk(int r) const { return reinterpret_cast<Walk*>(ws + r * ws_row(cells)); }
   __device__ __forceinline__ uint64_t* list(int r) const { return reinterpret_cast<uint64_t*>(walk(r) + 1); }
   __device__ __forceinline__ double* bins(int r) const { return reinterpret_cast<double*>(list(r) + SAMPLE_LIST); }
   __device__ __forceinline__ double* masses(int r) const { return bins(r) + SAMPLE_BINS; }
-  __device__ __forceinline__ float* maxima(int r) const { return reinterpret_cast<float*>(masses(r) + cells); }
+  __device__ __forceinline__ float* parts(int r) const { return reinterpret_cast<float*>(masses(r) + cells); }
+  __device__ __forceinline__ float* maxima(int r) const { return parts(r) + SAMPLE_PARTS; }
 };
 inline int sample_cells(int V) { return (V / 4 + SAMPLE_CELL - 1) / SAMPLE_CELL + 2; }  // at most, for any type and address
 
@@ -164,10 +169,10 @@ __device__ __forceinline__ float cell_max(float v) { return rotated_max<1>(rotat
 
 // ------------------------------------------------------------------------------------------------
 constexpr int SAMPLE_SHARES = 2048;  // workgroups of the second and third launch
-constexpr int SAMPLE_SPLIT = 256;  // threads of a workgroup that takes a part of a row
-template <typename T, int U>
+template <typename T>
 __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a) {
-  constexpr int E = Row<T>::E;
+  constexpr int E = Row<T>::E, U = SAMPLE_FIRST;
+  __shared__ float wm[SAMPLE_SPLIT / WAVE];
   const int row = blockIdx.y;
   const Row<T> x(a, row);
   const int nv = x.vectors(), v0 = blockIdx.x * (SAMPLE_SPLIT * U) + threadIdx.x;
@@ -176,6 +181,7 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a
   for (int u = 0; u < U; u++)
     if (v0 + u * SAMPLE_SPLIT < nv) x.load(v0 + u * SAMPLE_SPLIT, l[u]);
   float* out = a.maxima(row);
+  float all = -INFINITY;
 #pragma unroll
   for (int u = 0; u < U; u++) {
     const int v = v0 + u * SAMPLE_SPLIT;
@@ -186,6 +192,14 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_cells_kernel(SampleArgs a
     }
     m = cell_max(m);
     if (threadIdx.x % SAMPLE_CELL == 0 && v < nv) out[v / SAMPLE_CELL] = m;
+    all = fmaxf(all, m);
+  }
+  all = wave_max(all);
+  if (threadIdx.x % WAVE == 0) wm[threadIdx.x / WAVE] = all;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < SAMPLE_SPLIT / WAVE; i++) all = fmaxf(all, wm[i]);
+    a.parts(row)[blockIdx.x] = all;
   }
   // cleared for the next kernel to add to
   for (int i = blockIdx.x * SAMPLE_SPLIT + threadIdx.x; i < SAMPLE_BINS; i += gridDim.x * SAMPLE_SPLIT) a.bins(row)[i] = 0;
@@ -207,25 +221,28 @@ __device__ __forceinline__ void each_vector(const Row<T>& x, int v, int end, F&&
   }
 }
 
+// the row's largest logit, by every wave
+__device__ __forceinline__ float row_max(const SampleArgs& a, int row, int parts) {
+  const float* p = a.parts(row);
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SAMPLE_PARTS; i += WAVE) m = fmaxf(m, i + (int)(threadIdx.x % WAVE) < parts ? p[i + threadIdx.x % WAVE] : -INFINITY);
+  return wave_max(m);
+}
+
 template <typename T>
-__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a, int share) {
+__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a, int share, int parts) {
   constexpr int E = Row<T>::E;
   __shared__ double bins[SAMPLE_BINS];
-  __shared__ float wm[SAMPLE_SPLIT / WAVE];
   const int row = blockIdx.y, tid = threadIdx.x;
   const Row<T> x(a, row);
   const int cells = x.cells(), v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
   const Settings s(a, row, cells);
   if (s.kind != TOP_P && s.kind != ALL) return;
-  float m = -INFINITY;
-  const float* maxima = a.maxima(row);
-  for (int i = tid; i < cells; i += SAMPLE_SPLIT) m = fmaxf(m, maxima[i]);
-  m = wave_max(m);
-  if (tid % WAVE == 0) wm[tid / WAVE] = m;
-  for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT) bins[i] = 0;
+  if (s.kind == TOP_P)
+    for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT) bins[i] = 0.;
+  const Weights weight(row_max(a, row, parts), s.temperature);
   __syncthreads();
-  for (int i = 0; i < SAMPLE_SPLIT / WAVE; i++) m = fmaxf(m, wm[i]);
-  const Weights weight(m, s.temperature);
   each_vector(x, v0 + tid, v1, [&](int v, const float (&l)[E]) {  // (whole cells: shares and vectors() are multiples of 16)
     double sum = 0.;
 #pragma unroll
@@ -250,20 +267,17 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a,
 __device__ __forceinline__ uint64_t sample_rank(float l, int i) { return (uint64_t)~sample_key(l) << 32 | (unsigned)i; }
 
 template <typename T>
-__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a, int share) {
+__global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a, int share, int parts) {
   constexpr int E = Row<T>::E, WAVES = SAMPLE_SPLIT / WAVE, PER = SAMPLE_BINS / SAMPLE_SPLIT;
   __shared__ double wd[WAVES], found;
   __shared__ uint64_t list[SAMPLE_LIST];
-  __shared__ float wm[WAVES];
   __shared__ int found_bin, count, begin_at;
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
   const Row<T> x(a, row);
   const int cells = x.cells(), v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
   const Settings s(a, row, cells);
   if (s.kind != TOP_P) return;
-  float m = -INFINITY;
-  const float* maxima = a.maxima(row);
-  for (int i = tid; i < cells; i += SAMPLE_SPLIT) m = fmaxf(m, maxima[i]);
+  const Weights weight(row_max(a, row, parts), s.temperature);
   // the stretch of weights that the cut lies in
   double w[PER], sum = 0.;
 #pragma unroll
@@ -274,14 +288,11 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a,
     const double y = __shfl_up(upto, o, 64);
     if (lane >= o) upto += y;
   }
-  m = wave_max(m);
-  if (lane == 0) wm[wave] = m;
   if (tid == 0) count = 0;
   if (lane == WAVE - 1) wd[wave] = upto;
   __syncthreads();
   double all = 0.;
   for (int i = 0; i < WAVES; i++) {
-    m = fmaxf(m, wm[i]);
     upto += i < wave ? wd[i] : 0.;
     all += wd[i];
   }
@@ -306,7 +317,6 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a,
     out->goal = goal;
     out->bin = b;
   }
-  const Weights weight(m, s.temperature);
   each_vector(x, v0 + tid, v1, [&](int v, const float (&l)[E]) {
     double cell = 0.;
 #pragma unroll
@@ -840,19 +850,17 @@ inline bool sample_needs_mass(const SampleArgs& a) {  // whether any row may, fr
 
 template <typename T>
 void sample_launch(const SampleArgs& a, int B, hipStream_t st) {
-  // vectors a thread; us, one row of 128256 fp32, 256 rows: 2 14.3, 38.4; 4 15.1, 39.9; 8 16.6, 41.7
-  constexpr int U = 2;
-  const int vectors = a.V / Row<T>::E + 3 * SAMPLE_CELL;
-  const dim3 grid((vectors + SAMPLE_SPLIT * U - 1) / (SAMPLE_SPLIT * U), B);
-  sample_cells_kernel<T, U><<<grid, SAMPLE_SPLIT, 0, st>>>(a);
+  // vectors a thread of the first launch; us, one row of 128256 fp32, 256 rows: 2 14.3, 38.4; 4 15.1, 39.9; 8 16.6, 41.7
+  const int vectors = a.V / Row<T>::E + 3 * SAMPLE_CELL, first = (vectors + SAMPLE_SPLIT * SAMPLE_FIRST - 1) / (SAMPLE_SPLIT * SAMPLE_FIRST);
+  sample_cells_kernel<T><<<dim3(first, B), SAMPLE_SPLIT, 0, st>>>(a);
   if (sample_needs_mass(a)) {
     // a share's fixed work - the cells' maxima, the bins - is that of some thousand logits, so no more shares than fill the CUs; twice as
     // many where the settings are the rows' own, since only some rows need this then.  256 rows, 2048 : 4096, us: all with top-p 119 : 135,
     // settings of their own 90 : 84
     const int shares = SAMPLE_SHARES * (a.top_ks || a.top_ps || a.temperatures ? 2 : 1);
     const int parts = std::max(1, std::min((vectors + 4 * SAMPLE_SPLIT - 1) / (4 * SAMPLE_SPLIT), shares / B)), share = ((vectors + parts - 1) / parts + SAMPLE_CELL - 1) / SAMPLE_CELL * SAMPLE_CELL;
-    sample_mass_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share);
-    if (a.top_ps || a.top_p < 1.f) sample_walk_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share);
+    sample_mass_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share, first);
+    if (a.top_ps || a.top_p < 1.f) sample_walk_kernel<T><<<dim3(parts, B), SAMPLE_SPLIT, 0, st>>>(a, share, first);
   }
   sample_pick_kernel<T><<<B, SAMPLE_THREADS, 0, st>>>(a);
 }
