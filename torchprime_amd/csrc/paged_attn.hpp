@@ -6,8 +6,8 @@
 // calculation for softmax", 2018).  A key and its value are used by the g = Hq / Hkv query heads that share them: 2 g flops for
 // each element read, so it is the reading of the cache that bounds long calls, and the chain of dependent loads short ones.
 //
-// 16-bit and 8-bit caches (paged_attn_kernel): the g heads are the 16 columns of 16x16x32 matrix products (more than 16 heads: blocks
-// of 16, the unused columns zero), which costs a few percent of the time that the bytes take, whatever g is.  Layouts (lane: r = lane
+// paged_attn_kernel: the g heads are the 16 columns of 16x16x32 matrix products (fp32: 16x16x4; more than 16 heads: blocks of 16, the
+// unused columns zero), which costs a few percent of the time that the bytes take, whatever g is.  Layouts (lane: r = lane
 // % 16, g = lane / 16): A and B hold row / column r, k = 8 g + 0..7; C holds column r, rows 4 g + 0..3.  A wave takes 32 keys at a
 // time, straight from memory into the operands, without LDS and without an exchange between lanes:
 //   * scores are S^T = K Q^T, two products of 16 keys.  Row i of product t is key 8 (i / 4) + 4 t + i % 4, so that the scores of a
@@ -39,7 +39,8 @@ struct PagedAttnArgs {
 };
 
 // ------------------------------------------------------------------------------------------------
-// fp32: one workgroup per (sequence, query head): a thread takes a key of every 256, then a few columns of the values
+// fp32 heads of (192, 128), whose operands do not fit a wave's registers: one workgroup per (sequence, query head); a thread takes a
+// key of every 256, then a few columns of the values
 // ------------------------------------------------------------------------------------------------
 constexpr int PA_KEYS = 256;
 __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs a) {
@@ -186,6 +187,9 @@ __device__ __forceinline__ float* pa_piece(const PagedAttnArgs& a, int groups, i
 }
 
 template <typename T> struct MM;
+template <> struct MM<float> {
+  static __device__ __forceinline__ f32x4 dot(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+};
 template <> struct MM<bf16_t> {
   static __device__ __forceinline__ f32x4 dot(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ unsigned from_fp8(unsigned w, bool hi) {
@@ -226,13 +230,21 @@ template <int DV> struct Partial {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4 x) {
+  if constexpr (std::is_same<T, float>::value) *reinterpret_cast<f32x4*>(p) = x;
+  else *reinterpret_cast<u32x2*>(p) = pack4<T>(x[0], x[1], x[2], x[3]);
+}
+
 template <typename T, bool QUANT, int DQK, int DV>
 struct PagedTile {
-  typedef T v8 __attribute__((ext_vector_type(8)));
-  static constexpr int KS = DQK / 32;                 // products per 16 keys
-  static constexpr int KL = QUANT ? DQK / 64 : KS;    // 16-byte loads of a key per lane
+  static constexpr bool F32 = std::is_same<T, float>::value;
+  typedef T v8 __attribute__((ext_vector_type(F32 ? 4 : 8)));  // 16 bytes
+  static constexpr int B = QUANT ? 1 : sizeof(T);     // bytes of a cached element
+  static constexpr int KL = DQK * B / 64;             // 16-byte loads of a key per lane
+  static constexpr int KS = DQK / (F32 ? 16 : 32);    // 16-byte pieces of a query per lane
   static constexpr int C = DV / 16;                   // columns of V per lane
-  static constexpr int VB = C * (QUANT ? 1 : 2);      // their bytes
+  static constexpr int VB = C * B;                    // their bytes
   static constexpr bool RANGE = QUANT && std::is_same<T, f16_t>::value;
 
   static __device__ __forceinline__ void load_q(const PagedAttnArgs& a, const T* q, bool mine, v8 (&f)[KS]) {
@@ -240,7 +252,7 @@ struct PagedTile {
 #pragma unroll
     for (int i = 0; i < KS; i++) {
       // (8-bit keys: 16 bytes of a key, two products' shares, lie side by side)
-      const int d = QUANT ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+      const int d = QUANT ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 64 / B * i + 16 / B * g;
       f[i] = mine ? *reinterpret_cast<const v8*>(q + d) : v8{};
     }
   }
@@ -265,9 +277,8 @@ struct PagedTile {
   static __device__ __forceinline__ void load(const PagedAttnArgs& a, const Where& at, int kv, int key0, Data& x) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, mask = (1 << a.table.page_shift) - 1;
     const int tk = key0 + 8 * (r >> 2), tv = key0 + 8 * g;
-    constexpr int E = QUANT ? 1 : 2;
-    const char* kp = a.k.base + E * (max(at.pk, 0) * a.k.page + kv * a.k.head + ((tk & mask) + (r & 3)) * a.k.slot) + 16 * g;
-    const char* vp = a.v.base + E * (max(at.pv, 0) * a.v.page + kv * a.v.head + (tv & mask) * a.v.slot) + VB * r;
+    const char* kp = a.k.base + B * (max(at.pk, 0) * a.k.page + kv * a.k.head + ((tk & mask) + (r & 3)) * a.k.slot) + 16 * g;
+    const char* vp = a.v.base + B * (max(at.pv, 0) * a.v.page + kv * a.v.head + (tv & mask) * a.v.slot) + VB * r;
     if constexpr (QUANT) {
       const int64_t row = (((int64_t)max(at.pv, 0) * a.heads + kv) << a.table.page_shift) + (tv & mask);
       load_f<float, 8>(a.k.scale + row, x.ks);
@@ -276,16 +287,21 @@ struct PagedTile {
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int i = 0; i < KL; i++) x.k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + E * 4 * t * a.k.slot + 64 * i));
+      for (int i = 0; i < KL; i++) x.k[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + B * 4 * t * a.k.slot + 64 * i));
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      typedef unsigned row_t __attribute__((ext_vector_type(VB / 4)));
-      if constexpr (VB == 4) {
-        x.v[e][0] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(vp + E * e * a.v.slot));
-      } else {
-        const row_t w = __builtin_nontemporal_load(reinterpret_cast<const row_t*>(vp + E * e * a.v.slot));
+      constexpr int W = VB > 16 ? 16 : VB;  // bytes of a load
+      typedef unsigned row_t __attribute__((ext_vector_type(W / 4)));
 #pragma unroll
-        for (int i = 0; i < VB / 4; i++) x.v[e][i] = w[i];
+      for (int j = 0; j < VB / W; j++) {
+        const char* from = vp + B * e * a.v.slot + W * j;
+        if constexpr (W == 4) {
+          x.v[e][0] = __builtin_nontemporal_load(reinterpret_cast<const unsigned*>(from));
+        } else {
+          const row_t w = __builtin_nontemporal_load(reinterpret_cast<const row_t*>(from));
+#pragma unroll
+          for (int i = 0; i < W / 4; i++) x.v[e][W / 4 * j + i] = w[i];
+        }
       }
     }
     x.tv = tv;
@@ -302,14 +318,18 @@ struct PagedTile {
       f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KS; i++) {
-        u32x4 f;
-        if constexpr (QUANT) {
+        if constexpr (F32) {
+          const v8 f = __builtin_bit_cast(v8, x.k[t][i]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc = MM<T>::dot(f[e], q[i][e], acc);
+        } else if constexpr (QUANT) {
+          u32x4 f;
 #pragma unroll
           for (int w = 0; w < 4; w++) f[w] = MM<T>::from_fp8(x.k[t][i / 2][2 * (i % 2) + w / 2], w % 2);
+          acc = MM<T>::dot(__builtin_bit_cast(v8, f), q[i], acc);
         } else {
-          f = x.k[t][i];
+          acc = MM<T>::dot(__builtin_bit_cast(v8, x.k[t][i]), q[i], acc);
         }
-        acc = MM<T>::dot(__builtin_bit_cast(v8, f), q[i], acc);
       }
 #pragma unroll
       for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e];
@@ -357,15 +377,30 @@ struct PagedTile {
       p.c = cx;
     }
     const float m = p.m == -INFINITY ? 0.f : p.m;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      y[e] = fast_exp2(s[e] - m);
+      p.l += y[e];
+      if constexpr (RANGE) y[e] *= __builtin_amdgcn_ldexpf(x.vs[e], -p.c);
+      else if constexpr (QUANT) y[e] *= x.vs[e];
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int t = 0; t < C; t++) p.o[t] = MM<T>::dot(__uint_as_float(x.v[e][t]), y[e], p.o[t]);
+    } else {
+      add_values(x, y, p);
+    }
+  }
+
+  static __device__ __forceinline__ void add_values(const Data& x, const float (&y)[8], Partial<DV>& p) {
     v8 w, rest;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      float y = fast_exp2(s[e] - m);
-      p.l += y;
-      if constexpr (RANGE) y *= __builtin_amdgcn_ldexpf(x.vs[e], -p.c);
-      else if constexpr (QUANT) y *= x.vs[e];
-      w[e] = (T)y;
-      rest[e] = (T)(y - (float)w[e]);
+      w[e] = (T)y[e];
+      rest[e] = (T)(y[e] - (float)w[e]);
     }
     // values: column C r + t of the eight keys, paired from the rows as they came
     unsigned cols[8][C / 2];
@@ -407,7 +442,7 @@ __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, int b, int h0
     }
     if (result) {
       const float inv = l != 0.f ? 1.f / l : 0.f;
-      *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(a.out) + b * a.o_b + (h0 + row) * a.o_h + d) = pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+      store4(reinterpret_cast<T*>(a.out) + b * a.o_b + (h0 + row) * a.o_h + d, o * inv);
       if (d == 0 && a.lse) a.lse[(int64_t)b * a.Hq + h0 + row] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
     } else {
       *reinterpret_cast<f32x4*>(piece + 32 + row * DV + d) = o;
@@ -553,7 +588,7 @@ __global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs 
   if (!mine) return;
   const int h = s.h0 + row;
   const float inv = l != 0.f ? 1.f / l : 0.f;
-  *reinterpret_cast<u32x2*>(reinterpret_cast<T*>(a.out) + s.b * a.o_b + h * a.o_h + 4 * lane) = pack4<T>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  store4(reinterpret_cast<T*>(a.out) + s.b * a.o_b + h * a.o_h + 4 * lane, o * inv);
   if (lane == 0 && a.lse) a.lse[(int64_t)s.b * a.Hq + h] = l != 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
 }
 
@@ -562,6 +597,7 @@ __global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs 
 // workgroup (of more waves) takes a whole segment, no piece is left over and no second launch follows.
 //   us, one CU's waves 4 : 8, up to 512 keys: one sequence of 461 keys and 8 kv heads 8.95 : 8.83, 16 of 20 to 300 9.8 : 9.0,
 //   64 of 20 to 300 13.1 : 15.2: eight waves where the segments do not fill the CUs, four where they do.
+inline bool paged_tiles(const tp_kv_cache* c) { return c->dtype != TP_F32 || c->k_dim == c->v_dim; }
 struct PagedPlan {
   bool whole;
   int waves, groups, least;
@@ -576,7 +612,8 @@ inline PagedPlan paged_plan(const tp_kv_cache* c, int B, int Hq) {
 
 template <typename T, bool QUANT, int DQK, int DV>
 int paged_launch(const PagedAttnArgs& a, const PagedPlan& plan, hipStream_t st) {
-  constexpr int OCC = QUANT ? 3 : 2;  // (waves per SIMD)
+  // waves per SIMD; 8-bit keys of 192 spill a dozen registers at three, which costs less than a third wave gives (54.2 : 51.8 us)
+  constexpr int OCC = QUANT ? 3 : 2;
   const int lds = plan.waves * (32 + a.rows * (DV + 4)) * 4;
   const auto kern = !plan.whole                  ? paged_attn_kernel<T, QUANT, DQK, DV, PA_WAVES, OCC, false>
                     : plan.waves == PA_WHOLE_FEW ? paged_attn_kernel<T, QUANT, DQK, DV, PA_WHOLE_FEW, 2, true>
@@ -601,7 +638,7 @@ int paged_launch(const PagedAttnArgs& a, const PagedPlan& plan, hipStream_t st) 
 
 extern "C" size_t tp_paged_attn_workspace_bytes(const tp_kv_cache* c, int B, int Hq, int dtype) {
   using namespace tp;
-  if (check_cache(c, dtype, B, "tp_paged_attn_workspace_bytes") != TP_OK || Hq < 1 || Hq % c->heads || dtype == TP_F32) return 0;
+  if (check_cache(c, dtype, B, "tp_paged_attn_workspace_bytes") != TP_OK || Hq < 1 || Hq % c->heads || !paged_tiles(c)) return 0;
   const PagedPlan plan = paged_plan(c, B, Hq);
   return plan.whole ? 0 : plan.groups * (sizeof(SegmentCut) + sizeof(float) * 2 * pa_piece_floats(c->v_dim));
 }
@@ -628,7 +665,7 @@ extern "C" int tp_paged_attn(const tp_kv_cache* c, const void* q, const int32_t*
                         o_strides[1], B, Hq, c->heads, (rep + 15) / 16, std::min(rep, 16), soft_cap > 0.f ? sm_scale : sm_scale * LOG2E, soft_cap,
                         window_left};
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == TP_F32) {
+  if (!paged_tiles(c)) {
     paged_attn_rows_kernel<<<B * Hq, PA_KEYS, 0, st>>>(a);
     return check_launch("tp_paged_attn");
   }
@@ -637,10 +674,10 @@ extern "C" int tp_paged_attn(const tp_kv_cache* c, const void* q, const int32_t*
   int rc = TP_OK;
   kv_dispatch(dtype, c->dtype == TP_FP8, [&](auto t, auto quant) {
     typedef decltype(t) T;
-    if constexpr (!std::is_same<T, float>::value) {
-      constexpr bool Q = quant.value;
-      rc = c->k_dim == 64 ? paged_launch<T, Q, 64, 64>(a, plan, st) : c->k_dim == 128 ? paged_launch<T, Q, 128, 128>(a, plan, st) : paged_launch<T, Q, 192, 128>(a, plan, st);
-    }
+    constexpr bool Q = quant.value;
+    if (c->k_dim == 64) rc = paged_launch<T, Q, 64, 64>(a, plan, st);
+    else if (c->k_dim == 128) rc = paged_launch<T, Q, 128, 128>(a, plan, st);
+    else if constexpr (!std::is_same<T, float>::value) rc = paged_launch<T, Q, 192, 128>(a, plan, st);
   });
   return rc;
 }
