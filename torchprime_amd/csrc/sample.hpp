@@ -39,7 +39,7 @@ constexpr int SAMPLE_SPLIT = 256;     // threads of a workgroup that takes a par
 constexpr int SAMPLE_FIRST = 2;       // vectors per thread of the first launch
 constexpr int SAMPLE_PARTS = SAMPLE_CELLS * SAMPLE_CELL / (SAMPLE_SPLIT * SAMPLE_FIRST) + 1;
 constexpr int SAMPLE_LIST = 1024;     // tokens that are sorted at most
-constexpr int SAMPLE_TOP_K = 640;     // the list takes top-k up to half the cells, and this: about C log(1 / (1 - k / C)) of C cells' tokens
+constexpr int SAMPLE_TOP_K = 960;     // the largest top-k that goes by the list
 constexpr int SAMPLE_BINS = 2048;     // over weights from 1 down to 2^-36
 constexpr float SAMPLE_BIN = SAMPLE_BINS / 36.5f;
 
@@ -105,7 +105,7 @@ struct Settings {
     if (top_k <= 0 || top_k >= a.V) top_k = 0;
     if (!(temperature > 0.f) || top_k == 1 || top_p <= 0.f) kind = GREEDY;
     else if (a.V <= SAMPLE_LIST) kind = LIST;
-    else if (top_k) kind = top_k <= min(cells / 2, SAMPLE_TOP_K) ? TOP_K : DIGITS;
+    else if (top_k) kind = top_k <= SAMPLE_TOP_K ? TOP_K : DIGITS;
     else if (top_p < 1.f) kind = TOP_P;
     else kind = min_p > 0.f ? MIN_P : ALL;
   }
@@ -504,14 +504,25 @@ struct Picker {
   }
   __device__ __forceinline__ float listed(int at) const { return sample_logit(~(unsigned)(s.list[at] >> 32)); }
 
-  // A bound that at least k tokens reach: the k-th largest of the cells' maxima, rounded down to 1/1023 of their range.  A logit
-  // reaches it where !(scaled(l) < bound); that is monotone in l, and true for the largest whatever the range is.
+  // A bound that at least k tokens reach: the k-th largest of the cells' maxima, rounded down to 1/1023 of their range.  About
+  // C log(1 / (1 - k / C)) tokens of C cells reach it; where k is more than half the cells, the k-th largest of all logits in
+  // that range is taken instead, in a walk over the row.  A logit reaches the bound where !(scaled(l) < bound); that is monotone in l,
+  // and true for the largest whatever the range is.
   __device__ __forceinline__ float scaled(float l) const { return (l - least) * scale; }
   __device__ __forceinline__ float pivot(int k) const {
     static_assert(SAMPLE_THREADS == 1024, "a thread per step");
     int* counts = reinterpret_cast<int*>(s.mass);
-    for (int i = tid; i < cells; i += SAMPLE_THREADS)
-      if (s.maxima[i] > -INFINITY) atomicAdd(&counts[1023 - max(0, min(1023, (int)scaled(s.maxima[i])))], 1);
+    const auto count = [&](float l) {
+      if (l >= least) atomicAdd(&counts[1023 - max(0, min(1023, (int)scaled(l)))], 1);
+    };
+    if (2 * k <= cells) {
+      for (int i = tid; i < cells; i += SAMPLE_THREADS) count(s.maxima[i]);
+    } else {
+      visit([&](int, int, const float (&l)[E]) {
+#pragma unroll
+        for (int e = 0; e < E; e++) count(l[e]);
+      });
+    }
     __syncthreads();
     const int n = counts[tid];
     int upto = n;
@@ -525,7 +536,7 @@ struct Picker {
     for (int i = 0; i < wave; i++) upto += s.wi[i];
     if (upto >= k && upto - n < k) s.at = 1023 - tid;
     __syncthreads();
-    // (cells with anything in them may be fewer than k: then all tokens are taken, and the list may come out too long)
+    // (fewer than k may have been counted: then all tokens are taken, and the list may come out too long)
     return s.at > 1023 ? -INFINITY : (float)s.at;
   }
 
