@@ -22,6 +22,7 @@ from .attention import AttentionModule, repeat_kv
 from .blocks import (DeepseekV3Attention, Llama4TextAttention, LlamaAttention, LlamaDecoderLayer, LlamaForCausalLM, LlamaModel,
                      MixtralAttention)
 from .config import Config
+from .generation import PagedKVCache, generate
 from .kernel_utils import SplashAttentionConfig, splash_attention_jax_wrapper, tpu_splash_attention_jax_call_wrapper
 from .llama4 import (
   Llama4TextL2Norm,
@@ -50,5 +51,5 @@ __all__ = [
   "MixtralRotaryEmbedding", "DeepseekV3RotaryEmbedding", "rotate_half", "apply_rotary_pos_emb",
   "apply_rotary_pos_emb_interleave", "LlamaAttention", "MixtralAttention", "DeepseekV3Attention", "Llama4TextAttention", "LlamaDecoderLayer", "LlamaModel", "LlamaForCausalLM", "Config",
   "Llama4TextL2Norm", "Llama4TextRotaryEmbedding", "apply_rotary_emb", "attn_temperature_scales", "apply_attn_temperature",
-  "cross_entropy_loss", "LlamaMLP", "add_rms_norm",
+  "cross_entropy_loss", "LlamaMLP", "add_rms_norm", "PagedKVCache", "generate",
 ]  # fmt: skip
