@@ -436,7 +436,9 @@ int tp_linears(const tp_linear_problem* problems, int count, int dtype, void* st
  * (page, head, slot) element strides.  dtype TP_BF16 / TP_F16 / TP_F32 stores rows as they are; TP_FP8 stores
  * e4m3(x * (448 / a)) with a = max |x| of the row and keeps a / 448 in k_scale / v_scale (pages, heads, page_size), contiguous
  * (rows with a < 2^-100 become zeros; rows with an infinity or a NaN read back as NaN).  A table entry outside [0, pages)
- * names no page: nothing is stored there, zeros are read, and attention leaves its positions out.
+ * names no page: nothing is stored there, zeros are read, and attention leaves its positions out.  table_width * page_size is at
+ * most 2^30.  k, v and the scales start at 16-byte addresses; strides keep rows 16-byte aligned (8 bytes in a TP_FP8 cache of head
+ * dims that are not multiples of 16).
  * ---------------------------------------------------------------------------------------------- */
 typedef struct tp_kv_cache {
   void *k, *v;

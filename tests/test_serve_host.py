@@ -35,8 +35,8 @@ CACHES = [
   (dict(k=None), -1, b"null"), (dict(table=None), -1, b"null"), (dict(pages=0), -1, b"positive"), (dict(heads=0), -1, b"positive"),
   (dict(page_size=12), -2, b"power of two"), (dict(page_size=4), -2, b"power of two"), (dict(k_dim=60), -2, b"head dim"),
   (dict(v_dim=520), -2, b"head dim"), (dict(dtype=_lib.TP_F16), -2, b"does not go"), (dict(dtype=_lib.TP_FP8), -1, b"k_scale"),
-  (dict(k_scale=16), -1, b"k_scale"), (dict(k_strides=[2048, 1024, 63]), -1, b"aligned"), (dict(v_strides=[-2048, 1024, 64]), -1, b"aligned"),
-  (dict(table_width=1 << 28), -2, b"2^31"), (dict(dtype=9), -2, b"does not go"),
+  (dict(k_scale=16), -1, b"k_scale"), (dict(k_scale=20), -1, b"16-byte"), (dict(k_strides=[2048, 1024, 63]), -1, b"aligned"), (dict(v_strides=[-2048, 1024, 64]), -1, b"aligned"),
+  (dict(table_width=1 << 28), -2, b"2^30"), (dict(dtype=9), -2, b"does not go"),
 ]  # fmt: skip
 
 

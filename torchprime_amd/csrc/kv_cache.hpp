@@ -221,7 +221,7 @@ inline int check_cache(const tp_kv_cache* c, int dtype, int B, const char* who) 
              "%s: a cache of dtype code %d does not go with tensors of code %d", who, c->dtype, dtype);
   TP_REQUIRE(B >= 1 && c->pages >= 1 && c->heads >= 1 && c->table_width >= 1 && c->table_stride >= 0, TP_ERR_BAD_ARG, "%s: sizes must be positive", who);
   TP_REQUIRE(c->page_size >= 8 && (c->page_size & (c->page_size - 1)) == 0, TP_ERR_UNSUPPORTED, "%s: page_size %d is not a power of two from 8 up", who, c->page_size);
-  TP_REQUIRE((int64_t)c->table_width * c->page_size <= 0x7fffffff, TP_ERR_UNSUPPORTED, "%s: the table covers more than 2^31 positions", who);
+  TP_REQUIRE((int64_t)c->table_width * c->page_size <= 1 << 30, TP_ERR_UNSUPPORTED, "%s: the table covers more than 2^30 positions", who);
   for (int d : {c->k_dim, c->v_dim})
     TP_REQUIRE(d >= 8 && d <= 512 && d % 8 == 0, TP_ERR_UNSUPPORTED, "%s: head dim %d is not a multiple of 8 up to 512", who, d);
   const int e = elem_size(c->dtype), step = c->dtype == TP_FP8 && !wide_lanes(c) ? 8 : 16;
@@ -229,6 +229,7 @@ inline int check_cache(const tp_kv_cache* c, int dtype, int B, const char* who) 
   for (int i = 0; i < 3; i++)
     TP_REQUIRE(c->k_strides[i] >= 0 && c->v_strides[i] >= 0 && c->k_strides[i] * e % step == 0 && c->v_strides[i] * e % step == 0, TP_ERR_BAD_ARG,
                "%s: strides of the cache must keep rows %d-byte aligned", who, step);
+  TP_REQUIRE((((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15) == 0, TP_ERR_BAD_ARG, "%s: the scales must start at 16-byte addresses", who);
   TP_REQUIRE((c->dtype == TP_FP8) == (c->k_scale != nullptr) && (c->dtype == TP_FP8) == (c->v_scale != nullptr), TP_ERR_BAD_ARG,
              "%s: an 8-bit cache needs k_scale and v_scale, another cache has none", who);
   return TP_OK;

@@ -145,7 +145,7 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
 }
 // Every wave works this out by itself; a lane counts ceil(B / 64) sequences.
 template <int UNIT>
-__device__ __forceinline__ Share share_of(const PagedAttnArgs& a, int groups, int least, int w) {
+__device__ __forceinline__ Share share_of(const PagedAttnArgs& a, int groups, int w) {
   const int lane = threadIdx.x & 63, each = (a.B + 63) / 64, segs = a.heads * a.blocks;
   const int b0 = min(lane * each, a.B), b1 = min(b0 + each, a.B);
   int n = 0, length = 0;
@@ -156,7 +156,7 @@ __device__ __forceinline__ Share share_of(const PagedAttnArgs& a, int groups, in
   const int upto = wave_scan(n, lane);
   Share s;
   s.total = __shfl(upto, 63, 64) * segs;
-  s.per = max(least, (s.total + groups - 1) / groups);
+  s.per = (s.total + groups - 1) / groups;
   const int u = w * s.per;
   s.b = s.at = s.length = 0;
   if (u >= s.total) return s;
@@ -456,7 +456,7 @@ __device__ __forceinline__ void join_parts(const PagedAttnArgs& a, int b, int h0
 
 // WHOLE: a workgroup per segment (few keys at most); otherwise equal shares of all units
 template <typename T, bool QUANT, int DQK, int DV, int WAVES, int OCC, bool WHOLE>
-__global__ __launch_bounds__(64 * WAVES, OCC) void paged_attn_kernel(PagedAttnArgs a, int least) {
+__global__ __launch_bounds__(64 * WAVES, OCC) void paged_attn_kernel(PagedAttnArgs a) {
   typedef PagedTile<T, QUANT, DQK, DV> Tile;
   constexpr int ROW = DV + 4;  // (heads 4 banks apart)
   constexpr int UNIT = WAVES * PA_TILE;
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void paged_attn_kernel(PagedAttnAr
     at = 0;  // (units are counted from the sequence's first)
     length = a.lengths[b];
   } else {
-    const Share s = share_of<UNIT>(a, gridDim.x, least, blockIdx.x);
+    const Share s = share_of<UNIT>(a, gridDim.x, blockIdx.x);
     per = s.per;
     u = blockIdx.x * per;
     u1 = min(u + per, s.total);
@@ -500,7 +500,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void paged_attn_kernel(PagedAttnAr
     Tile::load_q(a, reinterpret_cast<const T*>(a.q) + b * a.q_b + (h0 + r) * a.q_h, r < rows, q);
     Partial<DV> p;
     p.clear();
-    const int stop = min(keys.end, keys.base + step1 * UNIT);
+    const int stop = step1 == units ? keys.end : keys.base + step1 * UNIT;
     int key0 = keys.base + (step0 * WAVES + wave) * PA_TILE;
     typename Tile::Where at_keys = Tile::find(a, b, key0);
     for (; key0 < stop; key0 += UNIT) {
@@ -593,21 +593,21 @@ __global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs 
 }
 
 // ---- host --------------------------------------------------------------------------------------
-// Workgroups of a call and the least units each takes.  Where the table has room for no more than PA_WHOLE keys a sequence, a
+// Workgroups of a call, and their waves.  Where the table has room for no more than PA_WHOLE keys a sequence, a
 // workgroup (of more waves) takes a whole segment, no piece is left over and no second launch follows.
 //   us, one CU's waves 4 : 8, up to 512 keys: one sequence of 461 keys and 8 kv heads 8.95 : 8.83, 16 of 20 to 300 9.8 : 9.0,
 //   64 of 20 to 300 13.1 : 15.2: eight waves where the segments do not fill the CUs, four where they do.
 inline bool paged_tiles(const tp_kv_cache* c) { return c->dtype != TP_F32 || c->k_dim == c->v_dim; }
 struct PagedPlan {
   bool whole;
-  int waves, groups, least;
+  int waves, groups;
 };
-constexpr int PA_WAVES = 4, PA_WHOLE_FEW = 8, PA_CUS = 256, PA_GROUPS = 512, PA_GROUPS_8BIT = 768, PA_LEAST = 1, PA_WHOLE = 512;
+constexpr int PA_WAVES = 4, PA_WHOLE_FEW = 8, PA_CUS = 256, PA_GROUPS = 512, PA_GROUPS_8BIT = 768, PA_WHOLE = 512;
 inline PagedPlan paged_plan(const tp_kv_cache* c, int B, int Hq) {
   const int64_t segs = (int64_t)B * c->heads * ((Hq / c->heads + 15) / 16), keys = (int64_t)c->table_width * c->page_size;
-  if (keys <= PA_WHOLE) return {true, segs <= PA_CUS ? PA_WHOLE_FEW : PA_WAVES, (int)segs, 1};
+  if (keys <= PA_WHOLE) return {true, segs <= PA_CUS ? PA_WHOLE_FEW : PA_WAVES, (int)segs};
   const int64_t units = (keys + PA_TILE) / (PA_WAVES * PA_TILE) + 1, most = c->dtype == TP_FP8 ? PA_GROUPS_8BIT : PA_GROUPS;
-  return {false, PA_WAVES, (int)std::min(most, (segs * units + PA_LEAST - 1) / PA_LEAST), PA_LEAST};
+  return {false, PA_WAVES, (int)std::min(most, segs * units)};
 }
 
 template <typename T, bool QUANT, int DQK, int DV>
@@ -622,7 +622,7 @@ int paged_launch(const PagedAttnArgs& a, const PagedPlan& plan, hipStream_t st) 
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     TP_REQUIRE(e == hipSuccess, TP_ERR_LAUNCH, "tp_paged_attn: hipFuncSetAttribute failed: %s", hipGetErrorString(e));
   }
-  kern<<<plan.groups, 64 * plan.waves, lds, st>>>(a, plan.least);
+  kern<<<plan.groups, 64 * plan.waves, lds, st>>>(a);
   if (!plan.whole && plan.groups > 1) {
     const int per_row = PA_JOIN / (DV / 4);
     // many workgroups to a segment: eight threads share out the pieces of four columns
