@@ -39,6 +39,7 @@ constexpr int SAMPLE_SPLIT = 256;     // threads of a workgroup that takes a par
 constexpr int SAMPLE_FIRST = 2;       // vectors per thread of the first launch
 constexpr int SAMPLE_PARTS = SAMPLE_CELLS * SAMPLE_CELL / (SAMPLE_SPLIT * SAMPLE_FIRST) + 1;
 constexpr int SAMPLE_LIST = 1024;     // tokens that are sorted at most
+constexpr int SAMPLE_COUNTED = 128;   // tokens that are compared with each other at most; more are sorted
 constexpr int SAMPLE_TOP_K = 960;     // the largest top-k that goes by the list
 constexpr int SAMPLE_BINS = 2048;     // over weights from 1 down to 2^-36
 constexpr float SAMPLE_BIN = SAMPLE_BINS / 36.5f;
@@ -350,6 +351,8 @@ struct PickLds {
   float maxima[SAMPLE_CELLS];
   unsigned short chosen[SAMPLE_CELLS];
   uint64_t list[SAMPLE_LIST];
+  double weight[SAMPLE_COUNTED], sums[2][SAMPLE_COUNTED];
+  int ranks[SAMPLE_COUNTED];
   double wd[SAMPLE_WAVES];
   float most[SAMPLE_WAVES], least[SAMPLE_WAVES];
   int wi[SAMPLE_WAVES];
@@ -381,23 +384,6 @@ __device__ __forceinline__ double group_scan(double v, PickLds& s, double& all) 
 
 // list[0, n) in rising order; places from n to the next power of two are filled up
 __device__ __forceinline__ void sort_list(PickLds& s, int n) {
-  if (n <= WAVE) {  // (the usual case: one wave, in its registers)
-    if (threadIdx.x < WAVE) {
-      const int lane = threadIdx.x;
-      uint64_t x = lane < n ? s.list[lane] : ~0ull;
-#pragma unroll
-      for (int k = 2; k <= WAVE; k *= 2)
-#pragma unroll
-        for (int j = k / 2; j > 0; j /= 2) {
-          const uint64_t y = __shfl_xor((unsigned long long)x, j, 64);
-          const bool lower = (lane & j) == 0, rising = (lane & k) == 0;
-          x = (lower == rising) == (x < y) ? x : y;
-        }
-      s.list[lane] = x;
-    }
-    __syncthreads();
-    return;
-  }
   int size = 2 * WAVE;
   while (size < n) size *= 2;
   for (int i = n + threadIdx.x; i < size; i += SAMPLE_THREADS) s.list[i] = ~0ull;
@@ -448,6 +434,7 @@ struct Picker {
     }
     if (tid == 0) {
       s.count = s.cells = 0;
+      s.begin = 0.;
       s.at = 0x7fffffff;
     }
     reinterpret_cast<int*>(s.mass)[tid] = 0;  // (the counts of pivot)
@@ -555,36 +542,79 @@ struct Picker {
     return s.last;
   }
 
-  // The same cut and draw of up to 64 unsorted tokens by one wave: a lane adds up what ranks before its token, then what is kept and
-  // comes before it by index, taking all tokens in turn.
-  __device__ __forceinline__ void draw_few(const Weights& weight, int n, int k) const {
-    const uint64_t token = lane < n ? s.list[lane] : ~0ull;
-    const float y = lane < n ? weight(listed(lane)) : 0.f;
-    const double w = (double)y;
-    const auto of_lane = [](double v, int i) {
-      const uint64_t u = __builtin_bit_cast(uint64_t, v);
-      return __builtin_bit_cast(double, (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(u >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)u, i));
-    };
-    int rank = 0;
-    double before = 0.;
-    for (int i = 0; i < n; i++) {
-      const uint64_t other = (uint64_t)(unsigned)__builtin_amdgcn_readlane((int)(token >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)token, i);
-      const double v = of_lane(w, i);
-      rank += other < token;
-      before += other < token ? v : 0.;
+  // The same for a list in any order, of up to SAMPLE_COUNTED tokens, by comparing all with all: a thread adds up what a share of the
+  // list puts before its token, and the shares of a token meet in LDS (sums are exact).  That has fewer steps that wait for each
+  // other than a sort, but reads LDS n^2 / 64 times: one row with top-k 50, of which 52 tokens are listed, 14.1 us sorted and 11.8
+  // counted; 256 rows with top-k 200 (230 tokens) 46.9 and 48.1.
+  __device__ __forceinline__ int mine(int n, int& part, int& parts) const {
+    int size = WAVE;
+    while (size < n) size *= 2;
+    part = tid / size;
+    parts = SAMPLE_THREADS / size;
+    return tid & (size - 1);
+  }
+  __device__ __forceinline__ void count_ranks(const Weights& weight, int n) const {
+    if (tid < n) {
+      s.weight[tid] = (double)weight(listed(tid));
+      s.sums[0][tid] = s.sums[1][tid] = 0.;
+      s.ranks[tid] = 0;
     }
-    const bool in = lane < n && (k == 0 || rank < k);
-    const double all = wave_sum_f64(in ? w : 0.), goal = set.top_p < 1.f ? (double)set.top_p * all : INFINITY;
-    const double kept = in && (rank == 0 || before < goal) && y >= set.min_p ? w : 0.;
-    const int index = (int)(unsigned)token;
-    double upto = kept, mass = 0.;
-    for (int i = 0; i < n; i++) {
-      const double v = of_lane(kept, i);
-      upto += __builtin_amdgcn_readlane(index, i) < index ? v : 0.;
-      mass += v;
+    __syncthreads();
+    int part, parts;
+    const int i = mine(n, part, parts);
+    if (i < n) {
+      const uint64_t token = s.list[i];
+      int rank = 0;
+      double before = 0.;
+      for (int j = part; j < n; j += parts) {
+        const bool first = s.list[j] < token;
+        rank += first;
+        before += first ? s.weight[j] : 0.;
+      }
+      atomicAdd(&s.ranks[i], rank);
+      atomicAdd(&s.sums[0][i], before);
     }
+    __syncthreads();
+  }
+  __device__ __forceinline__ uint64_t cut_counted(const Weights& weight, int n, double before, double goal) const {
+    count_ranks(weight, n);
+    const bool kept = tid < n && (s.ranks[tid] == 0 || before + s.sums[0][tid] < goal);
+    // the last one kept is the one that as many are kept before as its rank says
+    const int many = __syncthreads_count(kept);
+    if (kept && s.ranks[tid] == many - 1) s.last = s.list[tid];
+    __syncthreads();
+    return s.last;
+  }
+  __device__ __forceinline__ void draw_counted(const Weights& weight, int n, int k) const {
+    count_ranks(weight, n);
+    const double w = tid < n ? s.weight[tid] : 0.;
+    const bool in = tid < n && (k == 0 || s.ranks[tid] < k);
+    double goal = INFINITY;
+    if (set.top_p < 1.f) {
+      double all;
+      group_scan(in ? w : 0., s, all);
+      goal = (double)set.top_p * all;
+    }
+    const double kept = in && (s.ranks[tid] == 0 || s.sums[0][tid] < goal) && (float)w >= set.min_p ? w : 0.;
+    if (tid < n) s.weight[tid] = kept;
+    __syncthreads();
+    int part, parts;
+    const int i = mine(n, part, parts);
+    double mass = 0.;
+    if (i < n) {
+      const unsigned index = (unsigned)s.list[i];
+      double before = 0.;
+      for (int j = part; j < n; j += parts) {
+        before += (unsigned)s.list[j] < index ? s.weight[j] : 0.;
+        mass += s.weight[j];
+      }
+      atomicAdd(&s.sums[1][i], before);
+      if (i == 0) atomicAdd(&s.begin, mass);
+    }
+    __syncthreads();
+    mass = s.begin;
     const double drawn = (double)fminf(fmaxf(a.uniform[row], 0.f), 0x1.fffffep-1f) * mass;
-    if (kept > 0. && upto > drawn && upto - kept <= drawn) answer(index, kept, mass);
+    if (tid < n && kept > 0. && s.sums[1][tid] <= drawn && s.sums[1][tid] + kept > drawn) answer((int)(unsigned)s.list[tid], kept, mass);
   }
 
   // Draws from the list (`n` sorted by rank, those up to `last` kept)
@@ -819,10 +849,7 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
     }, cells);
     __syncthreads();
     const int n = lds.count;
-    if (n <= WAVE) {
-      if (p.wave == 0) p.draw_few(weight, n, set.top_k);
-      return;
-    }
+    if (n <= SAMPLE_COUNTED) return p.draw_counted(weight, n, set.top_k);
     if (n <= SAMPLE_LIST) {
       sort_list(lds, n);
       return p.draw_listed(weight, n, p.cut(weight, n, set.top_k, 0., -1.));
@@ -838,8 +865,12 @@ __global__ __launch_bounds__(SAMPLE_THREADS) void sample_pick_kernel(SampleArgs 
       for (int c = p.tid; c < p.cells; c += SAMPLE_THREADS) lds.mass[c] = a.masses(p.row)[c];
       if (p.tid < n) lds.list[p.tid] = a.list(p.row)[p.tid];
       __syncthreads();
-      sort_list(lds, n);
-      last = p.cut(weight, n, 0, walk.before, walk.goal);
+      if (n <= SAMPLE_COUNTED) {
+        last = p.cut_counted(weight, n, walk.before, walk.goal);
+      } else {
+        sort_list(lds, n);
+        last = p.cut(weight, n, 0, walk.before, walk.goal);
+      }
       if (p.tid < n && lds.list[p.tid] <= last) {
         const float y = weight(p.listed(p.tid));
         if (y >= set.min_p) atomicAdd(&lds.mass[p.x.cell_of((int)(unsigned)lds.list[p.tid])], (double)y);
