@@ -11,6 +11,7 @@ torchprime.rope.rope                   :mod:`torchprime_amd.rope`
 RMSNorm / rotary classes and apply     :mod:`torchprime_amd.norm`, :mod:`torchprime_amd.rotary`
 functions in model/{llama,mixtral,
 deepseek_v3}/model.py
+none: it trains only                   :mod:`torchprime_amd.generation` (PagedKVCache, generate)
 =====================================  =============================================================
 
 Compute runs only in ``libtprime_hip.so`` (hand-written HIP kernels reached through the ``tprime`` operators of

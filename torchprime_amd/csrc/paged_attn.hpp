@@ -15,6 +15,13 @@
 //   * for V^T a lane needs 8 keys of one column, memory holds columns side by side: a lane loads the same DV / 16 columns of its 8
 //     keys, pairs the keys' halves with one v_perm per two elements, and product t takes column DV / 16 * r + t.  A row of values is
 //     read in one instruction by the 16 lanes of a group, and a lane ends with DV / 4 neighbouring columns of its head.
+//
+// Measured (8 kv heads of 128, 32 query heads, bfloat16 unless said): one sequence of 131072 keys 92 us = 5.8 TB/s; 128 sequences of 512
+// to 8192 263 us = 6.1 TB/s, in 8 bits 155 us = 5.4 TB/s; 128 heads of (192, 128), float16, up to 1537 keys 67 us = 4.7 TB/s; one
+// sequence of 461 keys 8.8 us.  In the long ones the workgroups of a round keep 26 MB on their way and a tile takes 4 us, which is the
+// memory's rate; around that stand the launch and the chain lengths -> table -> keys of the first tile (about 2 us), and the join (4 to
+// 5 us with its launch).  The short ones are that chain, and what one CU can load.  Loading a wave's next tile into registers while it
+// works on one was slower everywhere (118 against 92 us at 131072 keys: 256 registers and spills; 9.4 against 8.8 at 461).
 #pragma once
 #include "attn_common.hpp"
 #include "kv_cache.hpp"
@@ -598,6 +605,9 @@ __global__ __launch_bounds__(PA_JOIN) void paged_attn_join_kernel(PagedAttnArgs 
 //   us, one CU's waves 4 : 8, up to 512 keys: one sequence of 461 keys and 8 kv heads 8.95 : 8.83, 16 of 20 to 300 9.8 : 9.0,
 //   64 of 20 to 300 13.1 : 15.2: eight waves where the segments do not fill the CUs, four where they do.
 inline bool paged_tiles(const tp_kv_cache* c) { return c->dtype != TP_F32 || c->k_dim == c->v_dim; }
+// Shares: workgroups of four waves, as many as are resident.  us, waves a workgroup x workgroups, at 131072 keys, 128 long sequences in
+// bfloat16, in 8 bits: 8 x 256 90.6, 268, 186; 8 x 512 96.9, 275, 191; 4 x 512 93.5, 263, 177; 4 x 768 (three waves per SIMD) 96.5, 261,
+// 157; 2 x 1024 97.5, 263, 175; 4 x 1024 128, 349, 214 (128 registers).
 struct PagedPlan {
   bool whole;
   int waves, groups;

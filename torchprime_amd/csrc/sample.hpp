@@ -18,9 +18,13 @@
 //                        cell, and a list of its tokens.
 //   sample_pick_kernel   a workgroup per row.  A short list of tokens decides: with top-k, those not below the k-th largest of the
 //                        cells' largest logits (at least k tokens are not), found in the few cells that hold any; with top-p, the list
-//                        above; with min-p, those that have the weight.  It is sorted by rank, cut, and drawn from.  Where it would not
-//                        fit (thousands of equals, top-k in the thousands), the cut is found digit by digit over an order-preserving
+//                        above; with min-p, those that have the weight.  It is ranked, cut, and drawn from.  Where it would not fit
+//                        (thousands of equals, top-k in the thousands), the cut is found digit by digit over an order-preserving
 //                        integer key of the logits, slower.
+//
+// Measured, rows of 128256 fp32 logits: one row with top-k 50 and top-p 0.95 11.9 us (3.1 + 8.9, the second a chain of some forty
+// dependent LDS and memory accesses), with top-p alone 29 us (3.0 + 5.9 + 7.2 + 13); 256 rows with top-k 38 us (25 us of it the first
+// launch, 5.3 TB/s), with top-p alone 118 us (the histogram's LDS atomics 39, the walk 36), with settings of their own 79 us.
 #pragma once
 #include <float.h>
 
