@@ -185,6 +185,42 @@ def test_scales_of_very_different_size_in_8_bits():
     check(**p)
 
 
+@pytest.mark.parametrize("dtype,cache", [(F16, None), (F16, FP8), (BF16, None), (F32, None)])
+def test_one_key_far_above_many(dtype, cache):
+  """60000 keys whose weights are 1.45 times float16's smallest step beside one of weight 1: each counts little, together 0.5 %."""
+  n, D = 60000, 64
+  p = problem(1, 4, 1, D, D, 64, [n], dtype, cache, garbage=False)
+  q = torch.zeros((1, 4, 1, D))
+  q[..., 0] = 1.0
+  p["q"] = q.to(dtype)
+  gap = 16.25
+  for c, s in ((p["kc"], p["ks"]), (p["vc"], p["vs"])):
+    if s is not None:
+      s.fill_(1.0)
+  for name, value in (("kc", 0.0), ("vc", 1.0)):
+    c = p[name]
+    (c.view(torch.uint8) if cache else c).copy_(torch.full(c.shape, value).to(c.dtype).view(torch.uint8) if cache else torch.full(c.shape, value))
+  row = torch.zeros(D)
+  row[0] = gap if cache is None else 16.0
+  where = (p["table"][0, 400], 0, 17)
+  (p["kc"].view(torch.uint8) if cache else p["kc"])[where] = row.to(p["kc"].dtype).view(torch.uint8) if cache else row.to(dtype)
+  (p["vc"].view(torch.uint8) if cache else p["vc"])[where] = 0
+  if cache:
+    p["ks"][where] = gap / 16.0
+  check(**p, sm_scale=1.0)
+
+
+def test_pages_before_the_window_may_be_gone():
+  p = problem(3, 8, 2, 128, 128, 16, [700, 130, 33], BF16)
+  for b, n in enumerate(p["lengths"]):
+    p["table"][b, : max(0, n - 1 - 100) // 16] = -1
+  check(**p, window=100)
+
+
+def test_thousands_of_sequences():
+  check(**problem(4100, 1, 1, 64, 64, 8, [b % 9 for b in range(4100)], BF16, garbage=False, width=70))
+
+
 def test_many_sequences_and_one_answer_for_the_same_call():
   p = problem(300, 8, 2, 64, 64, 16, [(37 * b) % 211 for b in range(300)], BF16)
   a = check(**p)

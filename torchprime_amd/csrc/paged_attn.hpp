@@ -221,7 +221,7 @@ __device__ __forceinline__ float groups_sum(float v) {
 }
 
 // What a wave has of a segment.  The maximum m is lazy: it moves only when a score exceeds it by more than 8 (log2 units), so that the
-// sums are rarely rescaled.  Weights (at most 2^8) go into the product as two numbers of type T, the rounded weight and the rest, so
+// sums are rarely rescaled.  Weights (at most 2^8; float16: 2^15) go into the product as two numbers of type T, the rounded weight and the rest, so
 // that nothing but the result is rounded to 16 bits; the second product costs less than the bytes leave room for.  In an 8-bit cache
 // they carry the value's scale, and for float16, whose range is short, relative to 2^c, c the largest exponent of a scale so far.
 template <int DV> struct Partial {
@@ -252,7 +252,10 @@ struct PagedTile {
   static constexpr int KS = DQK / (F32 ? 16 : 32);    // 16-byte pieces of a query per lane
   static constexpr int C = DV / 16;                   // columns of V per lane
   static constexpr int VB = C * B;                    // their bytes
-  static constexpr bool RANGE = QUANT && std::is_same<T, f16_t>::value;
+  static constexpr bool F16 = std::is_same<T, f16_t>::value, RANGE = QUANT && F16;
+  // float16: weights from 2^7 (2^15 where the maximum lags) down to its smallest step, 2^-31 of the largest, so that thousands of keys far
+  // below the maximum add up as they should
+  static constexpr float UP = F16 ? 7.f : 0.f;
 
   static __device__ __forceinline__ void load_q(const PagedAttnArgs& a, const T* q, bool mine, v8 (&f)[KS]) {
     const int g = (threadIdx.x & 63) >> 4;
@@ -383,7 +386,7 @@ struct PagedTile {
       p.m = m;
       p.c = cx;
     }
-    const float m = p.m == -INFINITY ? 0.f : p.m;
+    const float m = (p.m == -INFINITY ? 0.f : p.m) - UP;
     float y[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void paged_attn_kernel(PagedAttnAr
     p.l = groups_sum(p.l);
     if (r < rows) {
       if (g == 0) {
-        mine[r] = p.m;
+        mine[r] = p.m - Tile::UP;  // (what the weights are relative to)
         mine[16 + r] = p.l;
       }
       float* o = mine + 32 + r * ROW + (DV / 4) * g;
