@@ -386,25 +386,50 @@ __device__ __forceinline__ double group_scan(double v, PickLds& s, double& all) 
   return before + v;
 }
 
-// list[0, n) in rising order; places from n to the next power of two are filled up
+// the value of lane ^ J
+template <int J> __device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+  constexpr int CTRL = J == 1 ? 0xb1 : J == 2 ? 0x4e : J == 8 ? 0x128 : -1;  // quads' permutations, a row's half rotation
+  if constexpr (CTRL >= 0)
+    return (uint64_t)(unsigned)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, false) << 32 |
+           (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+  else
+    return __shfl_xor((unsigned long long)v, J, 64);
+}
+template <int J> __device__ __forceinline__ void sort_within(uint64_t& x, int tid, int k) {
+  if constexpr (J > 0) {
+    const uint64_t y = lane_xor<J>(x);
+    x = (((tid & J) == 0) == ((tid & k) == 0)) == (x < y) ? x : y;
+    sort_within<J / 2>(x, tid, k);
+  }
+}
+template <int K> __device__ __forceinline__ void sort_wave(uint64_t& x, int tid) {
+  if constexpr (K > 1) {
+    sort_wave<K / 2>(x, tid);
+    sort_within<K / 2>(x, tid, K);
+  }
+}
+// list[0, n) in rising order, bitonic, an element a thread; only distances from a wave up go through LDS
 __device__ __forceinline__ void sort_list(PickLds& s, int n) {
-  int size = 2 * WAVE;
+  const int tid = threadIdx.x;
+  int size = WAVE;
   while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += SAMPLE_THREADS) s.list[i] = ~0ull;
-  __syncthreads();
-  for (int k = 2; k <= size; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      const int i = threadIdx.x;
-      if (i < size / 2) {
-        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-        const uint64_t x = s.list[lo], y = s.list[hi];
-        if ((x > y) == ((lo & k) == 0)) {
-          s.list[lo] = y;
-          s.list[hi] = x;
-        }
-      }
+  uint64_t x = tid < n ? s.list[tid] : ~0ull;
+  if (tid < size) sort_wave<WAVE>(x, tid);
+  for (int k = 2 * WAVE; k <= size; k *= 2) {
+    for (int j = k / 2; j >= WAVE; j /= 2) {
       __syncthreads();
+      if (tid < size) s.list[tid] = x;
+      __syncthreads();
+      if (tid < size) {
+        const uint64_t y = s.list[tid ^ j];
+        x = (((tid & j) == 0) == ((tid & k) == 0)) == (x < y) ? x : y;
+      }
     }
+    if (tid < size) sort_within<WAVE / 2>(x, tid, k);
+  }
+  __syncthreads();
+  if (tid < size) s.list[tid] = x;
+  __syncthreads();
 }
 
 template <typename T>
@@ -455,15 +480,23 @@ struct Picker {
     a.logprobs[row] = (float)log(chosen / all);
   }
 
-  // f(cell, vector, its logits), every lane of a cell's 16 together: of all cells, or of the `n` chosen ones
+  // f(cell, vector, its logits), every lane of a cell's 16 together, the loads four at a time: of all cells, or of the `n` chosen ones
   template <typename F>
   __device__ __forceinline__ void visit(F&& f, int n = -1) const {
-    for (int i = tid / SAMPLE_CELL; i < (n < 0 ? cells : n); i += SAMPLE_THREADS / SAMPLE_CELL) {
-      const int c = n < 0 ? i : s.chosen[i];
-      const int v = c * SAMPLE_CELL + tid % SAMPLE_CELL;
-      float l[E];
-      x.load(v, l);
-      f(c, v, l);
+    constexpr int U = 4, STEP = SAMPLE_THREADS / SAMPLE_CELL;
+    const int end = n < 0 ? cells : n;
+    for (int i = tid / SAMPLE_CELL; i < end; i += U * STEP) {
+      float l[U][E];
+      int c[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (i + u * STEP < end) {
+          c[u] = n < 0 ? i + u * STEP : s.chosen[i + u * STEP];
+          x.load(c[u] * SAMPLE_CELL + tid % SAMPLE_CELL, l[u]);
+        }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (i + u * STEP < end) f(c[u], c[u] * SAMPLE_CELL + tid % SAMPLE_CELL, l[u]);
     }
   }
 
