@@ -19,8 +19,6 @@
 
 namespace tp {
 
-typedef unsigned char fp8_t;  // a float8_e4m3fn, moved as its bits
-
 // One 16-bit, 32-bit or 8-bit tensor of the cache: (page, head, slot) strides in elements, dim contiguous
 struct PageRows {
   char* base;

@@ -23,8 +23,8 @@
 //                        integer key of the logits, slower.
 //
 // Measured, rows of 128256 fp32 logits: one row with top-k 50 and top-p 0.95 11.9 us (3.1 + 8.9, the second a chain of some forty
-// dependent LDS and memory accesses), with top-p alone 29 us (3.0 + 5.9 + 7.2 + 13); 256 rows with top-k 38 us (25 us of it the first
-// launch, 5.3 TB/s), with top-p alone 118 us (the histogram's LDS atomics 39, the walk 36), with settings of their own 79 us.
+// dependent LDS and memory accesses), with top-p alone 27 us (3.0 + 5.9 + 7.2 + 11.3); 256 rows with top-k 37 us (25 us of it the
+// first launch, 5.3 TB/s), with top-p alone 114 us (the histogram's LDS atomics 39, the walk 36), with settings of their own 75 us.
 #pragma once
 #include <float.h>
 
@@ -581,8 +581,8 @@ struct Picker {
 
   // The same for a list in any order, of up to SAMPLE_COUNTED tokens, by comparing all with all: a thread adds up what a share of the
   // list puts before its token, and the shares of a token meet in LDS (sums are exact).  That has fewer steps that wait for each
-  // other than a sort, but reads LDS n^2 / 64 times: one row with top-k 50, of which 52 tokens are listed, 14.1 us sorted and 11.8
-  // counted; 256 rows with top-k 200 (230 tokens) 46.9 and 48.1.
+  // other than a sort, but reads LDS n^2 / 64 times: one row with top-k 50, of which 52 tokens are listed, 14.6 us sorted and 11.8
+  // counted; 256 rows with top-k 200 (230 tokens) 42.8 and 47.2.
   __device__ __forceinline__ int mine(int n, int& part, int& parts) const {
     int size = WAVE;
     while (size < n) size *= 2;
