@@ -10,7 +10,7 @@
 // which its last token (logit, index) describes; min-p is a bound on the weight itself.  The draw walks the kept tokens by index,
 // which needs no sort of the row: a sum per cell of the row (16 vectors of 16 bytes), then the cell that the drawn weight falls into.
 //
-// Up to four launches, the two in the middle only where a row may need them:
+// Up to four launches, the two in the middle only where a row may need them, the last one alone for rows of up to 1024 logits:
 //   sample_cells_kernel  the row split over workgroups: the largest logit of each cell.  It reads everything, once, and is bound by HBM.
 //   sample_mass_kernel   rows without top-k: the weight of each cell (no filter at all), or of each of 2048 stretches of the logit's
 //                        range (top-p): the row again, from the caches unless the batch is larger than they are.
@@ -448,9 +448,21 @@ struct Picker {
         set(args, blockIdx.x, cells) {
     m = -INFINITY;
     least = INFINITY;
+    // a row that fits the list has had no first launch
     const float* maxima = a.maxima(row);
+    const bool small = a.V <= SAMPLE_LIST;
+    if (small) {
+      visit([&](int c, int, const float (&l)[E]) {
+        float t = l[0];
+#pragma unroll
+        for (int e = 1; e < E; e++) t = fmaxf(t, l[e]);
+        t = cell_max(t);
+        if (tid % SAMPLE_CELL == 0) s.maxima[c] = t;
+      });
+      __syncthreads();
+    }
     for (int i = tid; i < cells; i += SAMPLE_THREADS) {
-      const float c = maxima[i];
+      const float c = small ? s.maxima[i] : maxima[i];
       s.maxima[i] = c;
       m = fmaxf(m, c);
       least = fminf(least, c > -INFINITY ? c : INFINITY);
@@ -622,18 +634,8 @@ struct Picker {
     __syncthreads();
     return s.last;
   }
-  __device__ __forceinline__ void draw_counted(const Weights& weight, int n, int k) const {
-    count_ranks(weight, n);
-    const double w = tid < n ? s.weight[tid] : 0.;
-    const bool in = tid < n && (k == 0 || s.ranks[tid] < k);
-    double goal = INFINITY;
-    if (set.top_p < 1.f) {
-      double all;
-      group_scan(in ? w : 0., s, all);
-      goal = (double)set.top_p * all;
-    }
-    const double kept = in && (s.ranks[tid] == 0 || s.sums[0][tid] < goal) && (float)w >= set.min_p ? w : 0.;
-    if (tid < n) s.weight[tid] = kept;
+  // Draws from list[0, n), n up to SAMPLE_COUNTED, in any order: weight[i] is a token's weight, 0 where it is not kept; sums[1] is zero
+  __device__ __forceinline__ void draw_by_index(int n) const {
     __syncthreads();
     int part, parts;
     const int i = mine(n, part, parts);
@@ -651,11 +653,35 @@ struct Picker {
     __syncthreads();
     mass = s.begin;
     const double drawn = (double)fminf(fmaxf(a.uniform[row], 0.f), 0x1.fffffep-1f) * mass;
-    if (tid < n && kept > 0. && s.sums[1][tid] <= drawn && s.sums[1][tid] + kept > drawn) answer((int)(unsigned)s.list[tid], kept, mass);
+    if (tid < n && s.weight[tid] > 0. && s.sums[1][tid] <= drawn && s.sums[1][tid] + s.weight[tid] > drawn)
+      answer((int)(unsigned)s.list[tid], s.weight[tid], mass);
+  }
+  __device__ __forceinline__ void draw_counted(const Weights& weight, int n, int k) const {
+    count_ranks(weight, n);
+    const double w = tid < n ? s.weight[tid] : 0.;
+    const bool in = tid < n && (k == 0 || s.ranks[tid] < k);
+    double goal = INFINITY;
+    if (set.top_p < 1.f) {
+      double all;
+      group_scan(in ? w : 0., s, all);
+      goal = (double)set.top_p * all;
+    }
+    const double kept = in && (s.ranks[tid] == 0 || s.sums[0][tid] < goal) && (float)w >= set.min_p ? w : 0.;
+    if (tid < n) s.weight[tid] = kept;
+    draw_by_index(n);
   }
 
   // Draws from the list (`n` sorted by rank, those up to `last` kept)
   __device__ __forceinline__ void draw_listed(const Weights& weight, int n, uint64_t last) const {
+    const int many = __syncthreads_count(tid < n && s.list[tid] <= last);
+    if (many <= SAMPLE_COUNTED) {  // (the first ones)
+      if (tid < many) {
+        const float w = weight(listed(tid));
+        s.weight[tid] = w >= set.min_p ? (double)w : 0.;
+        s.sums[1][tid] = 0.;
+      }
+      return draw_by_index(many);
+    }
     // by index: the kept ones only
     uint64_t mine = ~0ull;
     if (tid < n && s.list[tid] <= last && weight(listed(tid)) >= set.min_p) mine = (s.list[tid] << 32) | (s.list[tid] >> 32);
@@ -931,7 +957,7 @@ template <typename T>
 void sample_launch(const SampleArgs& a, int B, hipStream_t st) {
   // vectors a thread of the first launch; us, one row of 128256 fp32, 256 rows: 2 14.3, 38.4; 4 15.1, 39.9; 8 16.6, 41.7
   const int vectors = a.V / Row<T>::E + 3 * SAMPLE_CELL, first = (vectors + SAMPLE_SPLIT * SAMPLE_FIRST - 1) / (SAMPLE_SPLIT * SAMPLE_FIRST);
-  sample_cells_kernel<T><<<dim3(first, B), SAMPLE_SPLIT, 0, st>>>(a);
+  if (a.V > SAMPLE_LIST) sample_cells_kernel<T><<<dim3(first, B), SAMPLE_SPLIT, 0, st>>>(a);
   if (sample_needs_mass(a)) {
     // a share's fixed work - the cells' maxima, the bins - is that of some thousand logits, so no more shares than fill the CUs; twice as
     // many where the settings are the rows' own, since only some rows need this then.  256 rows, 2048 : 4096, us: all with top-p 119 : 135,
