@@ -89,6 +89,26 @@ def test_other_arguments():
     assert call() == status, lib.tp_last_error()
 
 
+def test_workspaces():
+  """What fits a workgroup per segment (up to 512 keys) needs none; beyond that it is asked for, and its absence refused."""
+  lib = _lib.load()
+  buf, p = _buffer()
+  s2 = (ctypes.c_int64 * 2)(128, 64)
+  short, long = _cache(p, table_width=32), _cache(p, table_width=33)
+  size = lambda c, dt=_lib.TP_BF16: lib.tp_paged_attn_workspace_bytes(ctypes.byref(c), 1, 2, dt)  # noqa: E731
+  assert size(short) == 0 and 0 < size(long) < 1 << 20
+  assert size(_cache(p, table_width=33, page_size=12)) == 0 and size(long, 7) == 0  # (refused anyway)
+  assert lib.tp_paged_attn(ctypes.byref(long), p, p, p, None, None, 1, 2, s2, s2, 0.1, -1, 0.0, _lib.TP_BF16, None) == -1
+  assert lib.tp_paged_attn(ctypes.byref(long), p, p, p, None, p + 4, 1, 2, s2, s2, 0.1, -1, 0.0, _lib.TP_BF16, None) == -1
+  assert b"workspace" in lib.tp_last_error()
+  huge = _cache(p, table_width=1 << 26)
+  assert size(huge) < 1 << 24  # (bounded by the workgroups, not by the keys)
+  assert lib.tp_paged_attn(ctypes.byref(_cache(p, table_width=1 << 26)), p, p, p, None, p, 1 << 10, 2, s2, s2, 0.1, -1, 0.0, _lib.TP_BF16, None) == -2
+  assert lib.tp_sample_workspace_bytes(0, 5) == 0 and lib.tp_sample_workspace_bytes(3, (1 << 18) + 1) == 0
+  assert lib.tp_sample_workspace_bytes(3, 128256) == 3 * lib.tp_sample_workspace_bytes(1, 128256) > 0
+  assert lib.tp_sample(p, p, None, None, None, None, 1.0, 0, 1.0, 0.0, p, p, None, 1, 8, 8, 2, None) == -1
+
+
 def _tensors(dev="cpu"):
   k = torch.zeros((2, 4, 3, 128), dtype=torch.bfloat16, device=dev)
   cache = torch.zeros((6, 4, 16, 128), dtype=torch.bfloat16, device=dev)

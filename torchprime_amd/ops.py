@@ -362,7 +362,10 @@ def paged_attention(
   them): (B,Hq,1,Dv).  A sequence of length 0 gets zeros.
 
   ``sm_scale=None`` means ``1/sqrt(Dv)``, as in ``attention``.  ``window_left``: only positions ``j >= lengths[b] - 1 -
-  window_left``.  ``soft_cap``: logits become ``cap * tanh(logits / cap)``."""
+  window_left``.  ``soft_cap``: logits become ``cap * tanh(logits / cap)``.  Slots without a token take no part, whatever lies
+  there; a NaN or an infinity among the values that do makes its column NaN or infinite.
+
+  The work is planned for as many positions as ``block_table`` is wide, so hand over no more of it than is used."""
   if soft_cap is not None and soft_cap <= 0:
     raise ValueError(f"soft_cap must be positive, got {soft_cap}")
   if window_left is not None and window_left < 0:
