@@ -197,7 +197,7 @@ def _quantise(x):
   top = x.abs().amax(-1)
   some = top >= TINY
   scale = torch.where(some, top / FP8_MAX, 0.0)
-  back = torch.where(some, torch.full_like(top, FP8_MAX) / top, 0.0)  # (a number over a tensor would be a reciprocal and a product)
+  back = torch.where(some, FP8_MAX / top, 0.0)
   return (x * back[..., None]).to(torch.float8_e4m3fn), scale
 
 
