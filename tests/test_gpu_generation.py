@@ -88,6 +88,22 @@ def test_the_same_numbers_give_the_same_tokens_and_an_end_ends():
   assert torch.equal(each[1:3], tokens[1:3])
 
 
+@pytest.mark.parametrize("vocab", [256, 40000])  # (the small table's own lookup, and the library's)
+@pytest.mark.parametrize("pad", [-1, -100, 2**40])
+@pytest.mark.parametrize("chunk", [None, 32])
+def test_what_is_behind_a_prompt_is_not_read(chunk, pad, vocab):
+  """Values that are no tokens behind the prompts change nothing, bit for bit."""
+  model = small_model(torch.bfloat16, vocab=vocab)
+  lengths = [5, 70, 33, 64]
+  ids = prompts(4, 75, vocab, 10)
+  draw = lambda ids: tpa.generate(model, ids, 6, prompt_lengths=lengths, temperature=0.0, prompt_chunk=chunk, return_logits=True)  # noqa: E731
+  want = draw(ids)
+  for b, n in enumerate(lengths):
+    ids[b, n:] = pad
+  got = draw(ids)
+  assert torch.isfinite(got[2]).all() and all(torch.equal(g, w) for g, w in zip(got, want))
+
+
 def test_refusals():
   model = small_model(torch.bfloat16, layers=1)
   ids = prompts(2, 8, 256, 8)

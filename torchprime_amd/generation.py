@@ -181,6 +181,10 @@ def generate(
 
   # the prompts: every piece's hidden states, of which a prompt's last one is kept
   ends = torch.tensor(lengths).to(device)
+  ids = input_ids[:, :S]
+  if min(lengths) < S:
+    # (what is behind a prompt may be no token at all: token 0 goes through the layers in its place)
+    ids = torch.where(torch.arange(S, device=device) < ends[:, None], ids, 0)
   last = None
   step = prompt_chunk or S
   for first in range(0, S, step):
@@ -188,7 +192,7 @@ def generate(
     counts = [min(max(length - first, 0), n) for length in lengths]
     cache.extend(counts)
     positions = torch.arange(first, first + n, device=device)[None].expand(B, n)
-    x, residual = _hidden(inner, input_ids[:, first : first + n], positions, cache, None if min(counts) == n else torch.tensor(counts, dtype=torch.int32).to(device), first)
+    x, residual = _hidden(inner, ids[:, first : first + n], positions, cache, None if min(counts) == n else torch.tensor(counts, dtype=torch.int32).to(device), first)
     h = x + residual
     row = (ends - 1 - first).clamp(0, n - 1)
     here = h[torch.arange(B, device=device), row]
