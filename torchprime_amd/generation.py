@@ -10,9 +10,10 @@ from __future__ import annotations
 import torch
 
 from . import ops
-from .blocks import LlamaForCausalLM
-from .linear import embed, project
-from .norm import add_rms_norm
+from .attention import AttentionModule
+from .blocks import LlamaAttention, LlamaDecoderLayer, LlamaForCausalLM, LlamaModel
+from .linear import _GLOBAL_HOOKS, embed, project
+from .norm import LlamaRMSNorm, add_rms_norm
 from .rotary import apply_rotary_pos_emb
 
 __all__ = ["PagedKVCache", "generate"]
@@ -115,6 +116,40 @@ class PagedKVCache:
     return ops.paged_attention(q, *cache, self.lengths, sm_scale, **scales, **extensions)
 
 
+# the methods that _hidden and generate stand in for
+_OWN = {
+  LlamaForCausalLM: ("forward", "_logits"), LlamaModel: ("forward", "deferred"), LlamaDecoderLayer: ("forward", "forward_deferred", "_one_call"),
+  LlamaAttention: ("forward",), AttentionModule: ("forward",), LlamaRMSNorm: ("forward",),
+}  # fmt: skip
+
+
+def _check_model(model) -> None:
+  """The model runs here with a cache in its attention, so some of its modules do not see a call of their own: one that has
+  to (forward hooks, another ``forward``, another class) is refused rather than passed by.  Projections, the MLP, the
+  embedding and the rotary module are called."""
+
+  def check(m, cls):
+    own = isinstance(m, cls) and all(getattr(type(m), n) is getattr(cls, n) and n not in m.__dict__ for n in _OWN[cls])
+    if not own or m._forward_hooks or m._forward_pre_hooks:
+      raise NotImplementedError(f"generate runs {cls.__name__} with a cache of its own: a {type(m).__name__} with another forward or with forward hooks would be passed by")
+
+  if not isinstance(model, LlamaForCausalLM):
+    raise TypeError(f"generate takes a LlamaForCausalLM, got {type(model).__name__}")
+  if _GLOBAL_HOOKS[0] or _GLOBAL_HOOKS[1]:
+    raise NotImplementedError("generate would pass by the forward hooks of all modules (torch.nn.modules.module.register_module_forward_hook)")
+  check(model, LlamaForCausalLM)
+  check(model.model, LlamaModel)
+  for layer in model.model.layers:
+    check(layer, LlamaDecoderLayer)
+    check(layer.self_attn, LlamaAttention)
+    check(layer.self_attn.attention_block, AttentionModule)
+    check(layer.input_layernorm, LlamaRMSNorm)
+    check(layer.post_attention_layernorm, LlamaRMSNorm)
+    if layer.self_attn.attention_block.plain_causal(1, None) is None:
+      raise NotImplementedError("generate's attention is causal, without dropout, in the order of the tokens (no load_balance_cp)")
+  check(model.model.norm, LlamaRMSNorm)
+
+
 def _hidden(model, ids: torch.Tensor, positions: torch.Tensor, cache: PagedKVCache, counts: torch.Tensor | None, first: int):
   """The decoder's last hidden states (before the final norm) of new tokens (batch, S) at ``positions`` (batch, S) as (x,
   residual), with their keys and values stored.  ``first``: the position of column 0 where S > 1."""
@@ -157,12 +192,12 @@ def generate(
   ``input_ids`` (batch, S) hold the prompts from the left, ``prompt_lengths`` of them each (None: S); what is behind is not
   read.  Settings are those of :func:`torchprime_amd.ops.sample`, numbers or one per sequence; temperature 0 is greedy.  After
   ``eos_token_id`` a sequence's tokens are -1.  ``prompt_chunk``: prompts go through in pieces of that many tokens.
-  ``generator``: a generator of the model's device for the draws.
+  ``generator``: a generator of the model's device for the draws.  A model whose decoder layers, attention or norms have forward
+  hooks or a ``forward`` of their own is refused: they would not see their calls.
 
   Returns the new tokens (batch, n <= max_new_tokens) and their log-probabilities in the distributions that they were drawn from;
   with ``return_logits`` also the logits (batch, n, vocabulary)."""
-  if not isinstance(model, LlamaForCausalLM):
-    raise TypeError(f"generate takes a LlamaForCausalLM, got {type(model).__name__}")
+  _check_model(model)
   if input_ids.dim() != 2 or input_ids.shape[1] < 1 or max_new_tokens < 1:
     raise ValueError("expected input_ids (batch, tokens) with at least one token, and max_new_tokens >= 1")
   B, S = input_ids.shape
