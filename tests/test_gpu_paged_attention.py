@@ -128,6 +128,29 @@ def test_soft_cap_and_scale(dtype, cache):
   check(**p, sm_scale=0.01)
 
 
+@pytest.mark.parametrize("Hq,H,Dk,Dv", [(8, 2, 64, 64), (8, 2, 128, 128), (4, 4, 192, 128)])
+@pytest.mark.parametrize("factor", [1.0, 0.05])
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1000.0, 1e5])
+def test_soft_cap_in_fp32(cap, factor, Hq, H, Dk, Dv):
+  """fp32 has no weights in 16 bits, and the soft cap adds errors relative to the logit, however large the cap is.  With S = scale *
+  max_j sum |q||k_j| >= |s_j|, a capped logit is off by (D + 8) 2^-23 S (its sum; the cap shrinks that) and by 2^-20 S: the division, a tanh of
+  2 units in the last place, three products and the difference to the maximum are 8 roundings of 2^-24, of at most 2 S.  Sums of n weights
+  and of weighted values, and the exponential, are off by (n + 64) 2^-24 of themselves."""
+  n = 130
+  p = problem(1, Hq, H, Dk, Dv, 16, [n], F32)
+  p["q"] = p["q"] * factor
+  out, _, lse, _ = formula(**p, cap=cap)
+  A = formula(**(p | dict(vc=p["vc"].abs())), cap=cap)[0]
+  t = torch.arange(n)
+  k = p["kc"][p["table"][0].long()[t // 16], :, t % 16].double().abs().repeat_interleave(Hq // H, 1)  # (n, Hq, D)
+  S = (k * p["q"][0, :, 0].double().abs()).sum(-1).amax(0)[:, None] / math.sqrt(Dv)  # (Hq, 1)
+  e = ((Dk + 8) * 2.0**-23 + 2.0**-20) * S
+  bound = 2.0**-24 * out[0].abs() + (2 * e[..., None] + (n + 64) * 2.0**-24) * A[0]
+  got, got_lse = ops.paged_attn(*(p[x].to(DEV) for x in ("q", "kc", "vc", "table")), torch.tensor([n], device=DEV), 1 / math.sqrt(Dv), -1, cap)
+  assert ((got[0].cpu().double() - out[0]).abs() <= bound).all()
+  assert ((got_lse[0].cpu().double() - lse[0]).abs() <= e + (n + 64) * 2.0**-24 + 2.0**-21 * (1 + lse[0].abs())).all()
+
+
 @pytest.mark.parametrize("dtype,cache", [(BF16, None), (F16, None), (F32, None), (BF16, FP8)])
 def test_peaked_and_growing_logits(dtype, cache):
   """Logits of several hundred, and a maximum that moves with every stretch of keys: the running maximum is taken along."""

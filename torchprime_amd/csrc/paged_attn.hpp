@@ -350,8 +350,9 @@ struct PagedTile {
       s[e] *= a.scale;
     }
     if (a.cap > 0.f) {
+      // (fast_tanh is off by 2^-23 of 1, which the cap multiplies: too much for fp32 where logits are small beside it)
 #pragma unroll
-      for (int e = 0; e < 8; e++) s[e] = a.cap * LOG2E * fast_tanh(s[e] / a.cap);
+      for (int e = 0; e < 8; e++) s[e] = a.cap * LOG2E * (F32 ? tanhf(s[e] / a.cap) : fast_tanh(s[e] / a.cap));
     }
     const bool whole = x.page && tv >= first && tv + 8 <= end;
     if (!__all(whole)) {
