@@ -238,3 +238,32 @@ def test_refusals():
     with pytest.raises(err):
       call()
   assert (kc == 0).all()
+
+
+def test_64_bit_integers_beyond_32_bits_name_nothing():
+  """Positions, pages, counts and lengths that an int32 does not hold are outside the cache, never another place in it."""
+  B, H, S, D, page, pages, big = 6, 2, 4, 64, 8, 20, 2**32
+  k, v = randn((B, H, S, D), 1, BF16), randn((B, H, S, D), 2, BF16)
+  kc, vc = new_cache(pages, H, page, D, BF16, seed=3), new_cache(pages, H, page, D, BF16, seed=4)
+  table = table_for(B, 3, pages, 5).long()
+  table[1, 0] += big
+  table[1, 1] -= big
+  positions = torch.tensor([big + 5, 6, -big + 2, 2**63 - 1, -(2**63), 2])
+  counts = torch.tensor([4, 4, 4, 4, 4, big + 1])
+  want_k, _ = stored(kc, None, k, table, positions, counts)
+  want_v, _ = stored(vc, None, v, table, positions, counts)
+  got = kc.to(DEV), vc.to(DEV)
+  ops.kv_cache_write(k.to(DEV), v.to(DEV), *got, table.to(DEV), positions.to(DEV), counts.to(DEV))
+  assert torch.equal(bits(got[0]), bits(want_k)) and torch.equal(bits(got[1]), bits(want_v))
+  # the sixth sequence's four tokens are the only ones that went in
+  assert torch.equal(want_k[table[5, 0], :, 2:6], k[5]) and int((want_k != kc).any(-1).sum()) == S * H
+  ops.kv_cache_write(k.to(DEV), v.to(DEV), *got, table.to(DEV), torch.full((B,), 2, device=DEV), torch.tensor([-big, -big + 3, 0, -1, -(2**63), 0], device=DEV))
+  assert torch.equal(bits(got[0]), bits(want_k))
+  lengths = torch.tensor([big + 1, 24, -big + 9, 2**63 - 1, -(2**63), big])
+  ko, _ = ops.kv_cache_read(got[0], got[1], table.to(DEV), lengths.to(DEV), 24)
+  for b, n in enumerate([24, 24, 0, 24, 0, 24]):
+    want = torch.zeros((H, 24, D), dtype=BF16)
+    for t in range(n):
+      if table[b, t // page] in range(pages):
+        want[:, t] = want_k[table[b, t // page], :, t % page]
+    assert torch.equal(ko[b].cpu(), want)

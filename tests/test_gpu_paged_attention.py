@@ -332,3 +332,15 @@ def test_refusals():
   ):  # fmt: skip
     with pytest.raises(err):
       call()
+
+
+def test_64_bit_integers_beyond_32_bits():
+  """Lengths beyond the table are the table's, pages that an int32 does not hold are none."""
+  p = problem(4, 8, 2, 128, 128, 8, [40, 40, 40, 40], BF16, garbage=False)
+  p["table"] = p["table"].long()
+  p["table"][0, 2] += 2**32
+  p["table"][3] -= 2**32
+  p["lengths"] = [2**32 + 1, -(2**32) + 7, 2**63 - 1, 40]
+  out, bound, _, _ = formula(**p)
+  got = ops.paged_attention(*(p[x].to(DEV) for x in ("q", "kc", "vc", "table")), torch.tensor(p["lengths"], device=DEV))
+  assert ((got.cpu().double() - out).abs() <= bound).all() and (got[[1, 3]] == 0).all() and (got[[0, 2]] != 0).any()

@@ -260,3 +260,18 @@ def test_refusals():
   ):  # fmt: skip
     with pytest.raises(err):
       call()
+
+
+def test_top_k_of_64_bits():
+  """A top-k that an int32 does not hold keeps all, as the number does; so do those far below zero."""
+  row, ks = randn((3000,), 21, F32, 1.5), [2**32 + 1, 2**32, 2**63 - 1, -(2**32) + 1, -(2**63), 3000]
+  w = kept_weights(row)
+  at = torch.argsort(w)[1500:].tolist()[:: 1500 // len(ks)][: len(ks)]
+  share = w / w.sum()
+  u = (share.cumsum(0) - share / 2)[at]
+  assert (share[at] > 4 * REL).all()
+  x = row.to(DEV).expand(len(ks), -1).contiguous()
+  tokens, _ = ops.sample(x, u.float().to(DEV), top_k=torch.tensor(ks, device=DEV))
+  assert tokens.tolist() == at
+  for k, want in zip(ks, at):
+    assert ops.sample(x[:1], u[at.index(want)][None].float().to(DEV), top_k=k)[0].tolist() == [want]

@@ -1506,10 +1506,14 @@ struct Cache {
   tp_kv_cache c{};
   Tensor table;  // keeps a copy alive
 };
+// int32, or int64 with what int32 does not hold at its ends: outside every cache, table and vocabulary, as the number itself is
+Tensor to_int32(const Tensor& t) {
+  return t.scalar_type() == at::kInt ? t : t.clamp((int64_t)INT32_MIN, (int64_t)INT32_MAX).to(at::kInt);
+}
 Tensor prep_int(const Tensor& t, int64_t B, const char* name) {
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == B, name, " must have shape (", B, ",), got (", t.sizes(), ")");
   TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64, got ", t.scalar_type());
-  return t.to(at::kInt).contiguous();
+  return to_int32(t).contiguous();
 }
 Cache prep_cache(const Tensor& k, const Tensor& v, const Tensor& table, int64_t B, const Tensor& k_scale, const Tensor& v_scale) {
   TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 4 && k.size(0) == v.size(0) && k.size(1) == v.size(1) && k.size(2) == v.size(2), "k_cache (", k.sizes(),
@@ -1527,7 +1531,7 @@ Cache prep_cache(const Tensor& k, const Tensor& v, const Tensor& table, int64_t 
     TORCH_CHECK_VALUE(s->is_contiguous() && s->sizes() == k.sizes().slice(0, 3), "the scales must be contiguous (", k.sizes().slice(0, 3), "), got (", s->sizes(), ")");
   }
   Cache r;
-  r.table = table.to(at::kInt);
+  r.table = to_int32(table);
   if (r.table.stride(1) != 1) r.table = r.table.contiguous();
   r.c.k = k.data_ptr();
   r.c.v = v.data_ptr();
