@@ -344,3 +344,32 @@ def test_64_bit_integers_beyond_32_bits():
   out, bound, _, _ = formula(**p)
   got = ops.paged_attention(*(p[x].to(DEV) for x in ("q", "kc", "vc", "table")), torch.tensor(p["lengths"], device=DEV))
   assert ((got.cpu().double() - out).abs() <= bound).all() and (got[[1, 3]] == 0).all() and (got[[0, 2]] != 0).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("Dk,Dv", [(64, 64), (128, 128), (192, 128)])
+@pytest.mark.parametrize("n", [50, 3000])
+@pytest.mark.parametrize("weights", ["equal", "any", "small"])
+def test_an_infinite_value_makes_its_column_infinite(weights, n, Dk, Dv, dtype):
+  """A positive weight times an infinity is one, also where the weight is 1 (two equal numbers split into a rounded one and no rest), or
+  2^-40 of the largest; infinities of both signs add up to NaN.  Nothing else changes."""
+  p = problem(1, 8, 2, Dk, Dv, 16, [n], dtype, garbage=False)
+  at = lambda t: (p["table"][0, t // 16], 0, t % 16)  # noqa: E731
+  if weights == "equal":
+    p["q"] = torch.zeros_like(p["q"])
+  if weights == "small":
+    p["q"] = torch.zeros_like(p["q"])
+    p["q"][..., 0] = 1.0
+    p["kc"][..., 0] = 0.0
+    for t in (17, 33):
+      p["kc"][at(t)][0] = -28.0
+  args = lambda: (*(p[x].to(DEV) for x in ("q", "kc", "vc", "table")), torch.tensor([n], device=DEV), 1.0 if weights == "small" else None)  # noqa: E731
+  clean = ops.paged_attention(*args())
+  inf = math.inf
+  want = clean.clone()
+  for t, col, x in ((17, 3, inf), (33, 7, -inf), (17, 9, inf), (33, 9, -inf), (17, Dv - 1, inf), (33, Dv - 1, inf)):
+    p["vc"][at(t)][col] = x
+    want[:, :4, :, col] = x if col != 9 else float("nan")
+  got = ops.paged_attention(*args())
+  assert torch.isfinite(clean).all()
+  assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(0.5, 1e4, -1e4), want.nan_to_num(0.5, 1e4, -1e4))

@@ -253,6 +253,7 @@ struct PagedTile {
   static constexpr int C = DV / 16;                   // columns of V per lane
   static constexpr int VB = C * B;                    // their bytes
   static constexpr bool F16 = std::is_same<T, f16_t>::value, RANGE = QUANT && F16;
+  static constexpr bool REST = !F32 && !QUANT;  // values may be infinite (e4m3 has no infinity), and a weight's rest 0
   // float16: weights from 2^7 (2^15 where the maximum lags) down to its smallest step, 2^-31 of the largest, so that thousands of keys far
   // below the maximum add up as they should
   static constexpr float UP = F16 ? 7.f : 0.f;
@@ -318,8 +319,8 @@ struct PagedTile {
     x.page = at.pv >= 0;
   }
 
-  // takes the keys of a tile that are in [first, end) into the sums
-  static __device__ __forceinline__ void add(const PagedAttnArgs& a, const v8 (&q)[KS], Data& x, int first, int end, Partial<DV>& p) {
+  // takes the keys of a tile that are in [first, end) into the sums; `halves`: see add_values
+  static __device__ __forceinline__ void add(const PagedAttnArgs& a, const v8 (&q)[KS], Data& x, int first, int end, bool halves, Partial<DV>& p) {
     const int tv = x.tv;
     // scores
     float s[8];
@@ -402,16 +403,23 @@ struct PagedTile {
 #pragma unroll
         for (int t = 0; t < C; t++) p.o[t] = MM<T>::dot(__uint_as_float(x.v[e][t]), y[e], p.o[t]);
     } else {
-      add_values(x, y, p);
+      add_values(x, y, halves, p);
     }
   }
 
-  static __device__ __forceinline__ void add_values(const Data& x, const float (&y)[8], Partial<DV>& p) {
+  // A positive weight times an infinity is one, a rest of 0 times it is NaN: a wave whose sums are not finite takes its keys again with each
+  // weight as two positive halves, for the columns where they are not (floored in float16, where a half might be 0).
+  static __device__ __forceinline__ void add_values(const Data& x, const float (&y)[8], bool halves, Partial<DV>& p) {
     v8 w, rest;
+    if (REST && halves) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      w[e] = (T)y[e];
-      rest[e] = (T)(y[e] - (float)w[e]);
+      for (int e = 0; e < 8; e++) w[e] = rest[e] = (T)(0.5f * (F16 && y[e] > 0.f ? fmaxf(y[e], 0x1p-20f) : y[e]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        w[e] = (T)y[e];
+        rest[e] = (T)(y[e] - (float)w[e]);
+      }
     }
     // values: column C r + t of the eight keys, paired from the rows as they came
     unsigned cols[8][C / 2];
@@ -510,33 +518,45 @@ __global__ __launch_bounds__(64 * WAVES, OCC) void paged_attn_kernel(PagedAttnAr
     typename Tile::v8 q[Tile::KS];
     Tile::load_q(a, reinterpret_cast<const T*>(a.q) + b * a.q_b + (h0 + r) * a.q_h, r < rows, q);
     Partial<DV> p;
-    p.clear();
     const int stop = step1 == units ? keys.end : keys.base + step1 * UNIT;
-    int key0 = keys.base + (step0 * WAVES + wave) * PA_TILE;
-    typename Tile::Where at_keys = Tile::find(a, b, key0);
-    for (; key0 < stop; key0 += UNIT) {
-      const typename Tile::Where now = at_keys;
-      at_keys = Tile::find(a, b, key0 + UNIT);  // (on its way before the loads of this tile)
-      typename Tile::Data x;
-      Tile::load(a, now, kv, key0, x);
-      Tile::add(a, q, x, keys.first, keys.end, p);
-    }
-    p.l = groups_sum(p.l);
-    if (r < rows) {
-      if (g == 0) {
-        mine[r] = p.m - Tile::UP;  // (what the weights are relative to)
-        mine[16 + r] = p.l;
+    for (bool again = false;; again = true) {
+      p.clear();
+      int key0 = keys.base + (step0 * WAVES + wave) * PA_TILE;
+      typename Tile::Where at_keys = Tile::find(a, b, key0);
+      for (; key0 < stop; key0 += UNIT) {
+        const typename Tile::Where now = at_keys;
+        at_keys = Tile::find(a, b, key0 + UNIT);  // (on its way before the loads of this tile)
+        typename Tile::Data x;
+        Tile::load(a, now, kv, key0, x);
+        Tile::add(a, q, x, keys.first, keys.end, again, p);
       }
-      float* o = mine + 32 + r * ROW + (DV / 4) * g;
-      const float up = Tile::RANGE ? __builtin_amdgcn_ldexpf(1.f, p.c) : 1.f;
-      constexpr int C = DV / 16;
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int t = 0; t < C; t += 4) {
-          f32x4 x{p.o[t][e], p.o[t + 1][e], p.o[t + 2][e], p.o[t + 3][e]};
-          *reinterpret_cast<f32x4*>(o + e * C + t) = x * up;
+      p.l = groups_sum(p.l);
+      float finite = 0.f;  // not, where one of this lane's sums is not
+      if (r < rows) {
+        if (g == 0) {
+          mine[r] = p.m - Tile::UP;  // (what the weights are relative to)
+          mine[16 + r] = p.l;
         }
+        float* o = mine + 32 + r * ROW + (DV / 4) * g;
+        const float up = Tile::RANGE ? __builtin_amdgcn_ldexpf(1.f, p.c) : 1.f;
+        constexpr int C = DV / 16;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int t = 0; t < C; t += 4) {
+            f32x4* out = reinterpret_cast<f32x4*>(o + e * C + t);
+            f32x4 x{p.o[t][e], p.o[t + 1][e], p.o[t + 2][e], p.o[t + 3][e]};
+            x *= up;
+            if (again) {
+              const f32x4 before = *out;
+#pragma unroll
+              for (int i = 0; i < 4; i++) x[i] = __builtin_isfinite(before[i]) ? before[i] : x[i];
+            }
+            *out = x;
+            finite += x[0] + x[1] + (x[2] + x[3]);
+          }
+      }
+      if (!Tile::REST || again || __all(__builtin_isfinite(finite))) break;
     }
     __syncthreads();
     const bool result = step0 == 0 && step1 == units;
