@@ -275,3 +275,52 @@ def test_top_k_of_64_bits():
   assert tokens.tolist() == at
   for k, want in zip(ks, at):
     assert ops.sample(x[:1], u[at.index(want)][None].float().to(DEV), top_k=k)[0].tolist() == [want]
+
+
+def special_rows(V, dtype):
+  """Rows in which most tokens are masked, or the logits' range is all that the type has."""
+  inf, nan, top, low = math.inf, math.nan, torch.finfo(dtype).max, torch.finfo(dtype).min
+  g = torch.Generator().manual_seed(V)
+  any_of = lambda n: torch.randperm(V, generator=g)[:n]  # noqa: E731
+  filled = lambda *parts: _filled(V, -inf, parts)  # noqa: E731
+  yield "one token", filled((any_of(1), 3.0))
+  yield "thirty tokens", filled((any_of(30), 2 * randn((30,), 1)))
+  yield "two thousand side by side", filled((torch.arange(V // 3, V // 3 + 2000), 2 * randn((2000,), 2)))
+  yield "the last twenty", filled((torch.arange(V - 20, V), randn((20,), 3)))
+  yield "between NaN", _filled(V, nan, [(any_of(V // 2), -inf), (any_of(40), randn((40,), 4))])
+  yield "three infinities", _filled(V, 1.0, [(any_of(V // 2), randn((V // 2,), 5)), (any_of(3), inf)])
+  yield "many infinities", _filled(V, -1.0, [(any_of(1500), inf)])
+  yield "infinities and nothing else", filled((any_of(7), inf))
+  yield "both ends of the range", filled((any_of(20), low), (any_of(5), top))
+  yield "the lowest value", filled((any_of(400), low))
+  yield "the largest value", _filled(V, low, [(any_of(1500), top)])
+
+
+def _filled(V, value, parts):
+  row = torch.full((V,), value)
+  for at, x in parts:
+    row[at] = x
+  return row
+
+
+SPECIAL_SETTINGS = [dict(), dict(top_k=50), dict(top_k=1000), dict(top_p=0.3713), dict(min_p=0.51), dict(top_k=300, top_p=0.3713),
+                    dict(temperature=0.5, top_p=0.6171, min_p=0.051), dict(top_k=1200, top_p=0.6171)]  # fmt: skip
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", [5000, 128256])
+@pytest.mark.parametrize("settings", SPECIAL_SETTINGS, ids=str)
+def test_masked_and_special_logits_of_large_vocabularies(settings, V, dtype):
+  for name, row in special_rows(V, dtype):
+    print(name, flush=True)
+    check_draws(row, 8, dtype, **settings)
+
+
+@pytest.mark.parametrize("V", [5000, 128256])
+@pytest.mark.parametrize("settings", SPECIAL_SETTINGS + [dict(temperature=0.0)], ids=str)
+def test_rows_of_nothing_in_large_vocabularies(settings, V):
+  x = torch.full((3, V), -math.inf)
+  x[1] = math.nan
+  x[2, V - 1] = 1.0
+  tokens, logprobs = ops.sample(x.to(DEV), torch.full((3,), 0.5, device=DEV), **settings)
+  assert tokens.tolist() == [-1, -1, V - 1] and logprobs.tolist() == [-math.inf, -math.inf, 0.0]

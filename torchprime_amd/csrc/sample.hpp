@@ -549,7 +549,8 @@ struct Picker {
     static_assert(SAMPLE_THREADS == 1024, "a thread per step");
     int* counts = reinterpret_cast<int*>(s.mass);
     const auto count = [&](float l) {
-      if (l >= least) atomicAdd(&counts[1023 - max(0, min(1023, (int)scaled(l)))], 1);
+      // (the range may be beyond fp32, or all infinities: NaN is step 0, which every logit from `least` up reaches)
+      if (l >= least) atomicAdd(&counts[1023 - (int)fminf(fmaxf(scaled(l), 0.f), 1023.f)], 1);
     };
     if (2 * k <= cells) {
       for (int i = tid; i < cells; i += SAMPLE_THREADS) count(s.maxima[i]);
