@@ -324,3 +324,13 @@ def test_rows_of_nothing_in_large_vocabularies(settings, V):
   x[2, V - 1] = 1.0
   tokens, logprobs = ops.sample(x.to(DEV), torch.full((3,), 0.5, device=DEV), **settings)
   assert tokens.tolist() == [-1, -1, V - 1] and logprobs.tolist() == [-math.inf, -math.inf, 0.0]
+
+
+@pytest.mark.parametrize("V", [1023, 1024, 1025, 1040])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=200), dict(top_k=1000), dict(top_p=0.6171), dict(min_p=0.051), dict(temperature=0.0)], ids=str)
+def test_around_the_rows_that_one_launch_takes(settings, V):
+  row = randn((V,), V, F32, 1.5)
+  if settings.get("temperature", 1.0) > 0:
+    return check_draws(row, 20, **settings)
+  x = row.to(DEV).expand(300, -1).contiguous()
+  assert (ops.sample(x, torch.rand(300, device=DEV), **settings)[0] == int(row.argmax())).all()

@@ -149,3 +149,11 @@ def test_shapes_with_fake_tensors():
     assert out.shape == (2, 8, 1, 128) and out.dtype == q.dtype and lse.shape == (2, 8, 1) and lse.dtype == torch.float32
     tokens, logprobs = ops.sample_op(logits, u, None, None, None, None, 1.0, 0, 1.0, 0.0)
     assert tokens.shape == logprobs.shape == (2,) and tokens.dtype == torch.int64 and logprobs.dtype == torch.float32
+
+
+def test_rows_that_one_launch_takes_need_next_to_no_workspace():
+  """Up to 1024 logits a row never leaves its workgroup: 65535 such rows asked for 1.6 GB, of which nothing was used."""
+  lib = _lib.load()
+  for V in (1, 50, 1024):
+    assert 0 < lib.tp_sample_workspace_bytes(65535, V) <= 64
+  assert lib.tp_sample_workspace_bytes(2, 1025) == 2 * lib.tp_sample_workspace_bytes(1, 1025) > 2 * 1025

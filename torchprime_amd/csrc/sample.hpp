@@ -975,7 +975,8 @@ void sample_launch(const SampleArgs& a, int B, hipStream_t st) {
 
 extern "C" size_t tp_sample_workspace_bytes(int B, int V) {
   using namespace tp;
-  return B < 1 || V < 1 || V > SAMPLE_MOST ? 0 : B * (size_t)SampleArgs::ws_row(sample_cells(V));
+  if (B < 1 || V < 1 || V > SAMPLE_MOST) return 0;
+  return V <= SAMPLE_LIST ? 16 : B * (size_t)SampleArgs::ws_row(sample_cells(V));  // (a row that fits the list stays in its workgroup)
 }
 
 extern "C" int tp_sample(const void* logits, const float* uniform, const float* temperatures, const int32_t* top_ks, const float* top_ps,
