@@ -64,8 +64,7 @@ struct SampleArgs {
   // and of the cells
   struct Walk {
     double before, goal;
-    int bin, count;
-    int64_t none;
+    int count;
   };
   static constexpr int64_t ws_row(int cells) { return (sizeof(Walk) + SAMPLE_LIST * 8 + SAMPLE_BINS * 8 + SAMPLE_PARTS * 4 + (int64_t)cells * 12 + 15) / 16 * 16; }
   __device__ __forceinline__ Walk* walk(int r) const { return reinterpret_cast<Walk*>(ws + r * ws_row(cells)); }
@@ -102,7 +101,7 @@ struct Settings {
   float temperature, top_p, min_p;
   int top_k;  // 0: all
   SampleKind kind;
-  __device__ __forceinline__ Settings(const SampleArgs& a, int row, int cells) {
+  __device__ __forceinline__ Settings(const SampleArgs& a, int row) {
     temperature = a.temperatures ? a.temperatures[row] : a.temperature;
     top_k = a.top_ks ? a.top_ks[row] : a.top_k;
     top_p = fminf(fmaxf(a.top_ps ? a.top_ps[row] : a.top_p, 0.f), 1.f);
@@ -241,8 +240,8 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_mass_kernel(SampleArgs a,
   __shared__ double bins[SAMPLE_BINS];
   const int row = blockIdx.y, tid = threadIdx.x;
   const Row<T> x(a, row);
-  const int cells = x.cells(), v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
-  const Settings s(a, row, cells);
+  const int v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
+  const Settings s(a, row);
   if (s.kind != TOP_P && s.kind != ALL) return;
   if (s.kind == TOP_P)
     for (int i = tid; i < SAMPLE_BINS; i += SAMPLE_SPLIT) bins[i] = 0.;
@@ -279,8 +278,8 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a,
   __shared__ int found_bin, count, begin_at;
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
   const Row<T> x(a, row);
-  const int cells = x.cells(), v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
-  const Settings s(a, row, cells);
+  const int v0 = blockIdx.x * share, v1 = min(v0 + share, x.vectors());
+  const Settings s(a, row);
   if (s.kind != TOP_P) return;
   const Weights weight(row_max(a, row, parts), s.temperature);
   // the stretch of weights that the cut lies in
@@ -320,7 +319,6 @@ __global__ __launch_bounds__(SAMPLE_SPLIT) void sample_walk_kernel(SampleArgs a,
   if (blockIdx.x == 0 && tid == 0) {
     out->before = found;
     out->goal = goal;
-    out->bin = b;
   }
   each_vector(x, v0 + tid, v1, [&](int v, const float (&l)[E]) {
     double cell = 0.;
@@ -445,7 +443,7 @@ struct Picker {
 
   __device__ __forceinline__ Picker(const SampleArgs& args, PickLds& lds)
       : a(args), s(lds), row(blockIdx.x), tid(threadIdx.x), lane(tid & 63), wave(tid >> 6), x(args, blockIdx.x), nv(x.vectors()), cells(x.cells()),
-        set(args, blockIdx.x, cells) {
+        set(args, blockIdx.x) {
     m = -INFINITY;
     least = INFINITY;
     // a row that fits the list has had no first launch
