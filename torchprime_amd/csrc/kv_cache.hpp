@@ -12,8 +12,9 @@
 // three dependent loads: position, table entry, row (small ones).  A lane moves 8 elements, or stores 16 of
 // an 8-bit cache where the head dims allow (4 prompts of 8192 tokens, 8 heads of 128: 51 : 43 us; reading back is better with 8, whose
 // stores lie side by side, 43 : 51); a row is a group of 4 to 64 lanes of one wave, where the row's maximum is taken with lane exchanges.
-// Measured, 8 heads of 128, bfloat16: 4 prompts of 8192 stored 46 us = 5.9 TB/s, read back 5.9 TB/s; in 8 bits 43 us (4.6 TB/s) and
-// 43 us (4.7 TB/s); the tokens of one step of 64 sequences 2.5 us, which is what an empty launch takes.
+// Measured, 8 heads of 128, bfloat16: 4 prompts of 8192 stored 46 us = 5.9 TB/s, read back 5.9 TB/s; in 8 bits 44 us (4.7 TB/s) and
+// 43 us (4.7 TB/s: pieces of 8 bytes on the 8-bit side); 4 of 4096 in fp32 51 us (5.3 TB/s) and 53 us (5.1 TB/s); the tokens of one step of
+// 64 sequences 2.5 us, which is what an empty launch takes.
 #pragma once
 #include "common.hpp"
 

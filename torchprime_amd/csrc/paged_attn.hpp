@@ -16,9 +16,10 @@
 //     keys, pairs the keys' halves with one v_perm per two elements, and product t takes column DV / 16 * r + t.  A row of values is
 //     read in one instruction by the 16 lanes of a group, and a lane ends with DV / 4 neighbouring columns of its head.
 //
-// Measured (8 kv heads of 128, 32 query heads, bfloat16 unless said): one sequence of 131072 keys 92 us = 5.8 TB/s; 128 sequences of 512
-// to 8192 263 us = 6.1 TB/s, in 8 bits 155 us = 5.4 TB/s; 128 heads of (192, 128), float16, up to 1537 keys 67 us = 4.7 TB/s; one
-// sequence of 461 keys 8.8 us.  In the long ones the workgroups of a round keep 26 MB on their way and a tile takes 4 us, which is the
+// Measured (8 kv heads of 128, 32 query heads, bfloat16 unless said): one sequence of 131072 keys 92 us = 5.8 TB/s, in 8 bits 59 us =
+// 4.7 TB/s, heads of 64 60 us = 4.4 TB/s (8 bits 44 us = 3.3 TB/s: loads of 8 and 4 bytes a lane for the values); 128 sequences of 512
+// to 8192 265 us = 6.1 TB/s, in 8 bits 157 us = 5.3 TB/s; 128 heads of (192, 128), float16, up to 1537 keys 68 us = 4.6 TB/s, in 8 bits 52 us =
+// 3.1 TB/s; fp32, 16384 keys 34 us = 3.9 TB/s; one sequence of 461 keys 9.0 us.  In the long ones the workgroups of a round keep 26 MB on their way and a tile takes 4 us, which is the
 // memory's rate; around that stand the launch and the chain lengths -> table -> keys of the first tile (about 2 us), and the join (4 to
 // 5 us with its launch).  The short ones are that chain, and what one CU can load.  Loading a wave's next tile into registers while it
 // works on one was slower everywhere (118 against 92 us at 131072 keys: 256 registers and spills; 9.4 against 8.8 at 461).
@@ -47,7 +48,8 @@ struct PagedAttnArgs {
 
 // ------------------------------------------------------------------------------------------------
 // fp32 heads of (192, 128), whose operands do not fit a wave's registers: one workgroup per (sequence, query head); a thread takes a
-// key of every 256, then a few columns of the values
+// key of every 256, then a few columns of the values.  Not split over the keys: 512 heads of up to 1537 keys 171 us = 3.7 TB/s, but one
+// sequence of 16384 with 32 heads, which are 32 workgroups, 1184 us = 0.6 TB/s
 // ------------------------------------------------------------------------------------------------
 constexpr int PA_KEYS = 256;
 __global__ __launch_bounds__(PA_KEYS) void paged_attn_rows_kernel(PagedAttnArgs a) {
@@ -221,8 +223,9 @@ __device__ __forceinline__ float groups_sum(float v) {
 }
 
 // What a wave has of a segment.  The maximum m is lazy: it moves only when a score exceeds it by more than 8 (log2 units), so that the
-// sums are rarely rescaled.  Weights (at most 2^8; float16: 2^15) go into the product as two numbers of type T, the rounded weight and the rest, so
-// that nothing but the result is rounded to 16 bits; the second product costs less than the bytes leave room for.  In an 8-bit cache
+// sums are rarely rescaled.  Weights (at most 2^8; float16: 2^15) go into the product as two numbers of type T, the rounded weight and the rest,
+// which are off by 2^-18 of the weight together in bfloat16 and 2^-24 in float16 (or half its smallest step), where the result's rounding is
+// off by 2^-9 and 2^-12; the second product costs less than the bytes leave room for.  In an 8-bit cache
 // they carry the value's scale, and for float16, whose range is short, relative to 2^c, c the largest exponent of a scale so far.
 template <int DV> struct Partial {
   float m, l;  // of this lane's head; l over this lane's keys
@@ -408,7 +411,8 @@ struct PagedTile {
   }
 
   // A positive weight times an infinity is one, a rest of 0 times it is NaN: a wave whose sums are not finite takes its keys again with each
-  // weight as two positive halves, for the columns where they are not (floored in float16, where a half might be 0).
+  // weight as two positive halves, for the columns where they are not (floored in float16, where a half might be 0).  To look for that
+  // costs a call 0.1 to 0.25 us; sums of the rests by themselves, which need no second pass, cost 0.4 to 0.6 in another 32 registers.
   static __device__ __forceinline__ void add_values(const Data& x, const float (&y)[8], bool halves, Partial<DV>& p) {
     v8 w, rest;
     if (REST && halves) {
